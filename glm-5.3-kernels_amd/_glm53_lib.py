@@ -39,6 +39,11 @@ EXPORTED = (
     "glm53_indexer_topk",
     "glm53_indexer_topk_next_n",
     "glm53_stream_probe",
+    "glm53_chunk_mla_workspace_bytes",
+    "glm53_chunk_mla",
+    "glm53_store_rope",
+    "glm53_verify_drafts_workspace_bytes",
+    "glm53_verify_drafts",
 )
 
 _lib = None
@@ -116,6 +121,18 @@ def load():
     L.glm53_indexer_topk_next_n.argtypes = [P, I64, P, I64, I64, I64, I64, P, I64, P, I64, P]
     L.glm53_stream_probe.restype = I
     L.glm53_stream_probe.argtypes = [I, P, P, I64, P]
+    L.glm53_chunk_mla_workspace_bytes.restype = I64
+    L.glm53_chunk_mla_workspace_bytes.argtypes = [I64, I64, I64]
+    L.glm53_chunk_mla.restype = I
+    L.glm53_chunk_mla.argtypes = [P, I64, I64, P, I, I64, I64, I64, I64, P, P, P, I64, I64, I64, I64, I64, D, P, I64,
+                                  P, I64, I64, P, P]
+    L.glm53_store_rope.restype = I
+    L.glm53_store_rope.argtypes = [P, I64, P, I64, P, I, P, I, I64, I, P, F, P, I64, I64, I64, I64, P, I, I64,
+                                   P, I64, I64, P, I64, I64, I64, P]
+    L.glm53_verify_drafts_workspace_bytes.restype = I64
+    L.glm53_verify_drafts_workspace_bytes.argtypes = [I64, I64]
+    L.glm53_verify_drafts.restype = I
+    L.glm53_verify_drafts.argtypes = [P, I64, I64, P, I64, P, I, I64, P, P, P, I64, I64, I64, P, I64, P, P, P]
     version = L.glm53_abi_version()
     if version != ABI_VERSION:
         raise ImportError(f"{LIB_PATH} has ABI version {version}, expected {ABI_VERSION}")

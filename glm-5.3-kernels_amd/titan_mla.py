@@ -360,6 +360,100 @@ def triton_mla_sparse_attention_pooled(
     return out
 
 
+def mla_chunk_attention_paged(
+    q: torch.Tensor,
+    kv_cache: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    sm_scale: float,
+    *,
+    out: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """Dense causal latent attention of a ragged chunk of new tokens over a
+    paged cache: prefill chunks, the tokens of a speculative step and single
+    decode tokens in one call, every cached position read (no indices).
+
+    Request r has the query tokens cu_seqlens_q[r] .. cu_seqlens_q[r + 1), the
+    last of its seq_lens[r] cached positions (they are in the cache already:
+    titan_kv.store_rope, titan_kv.store_int8).  Its i-th of n tokens attends
+    to positions j <= seq_lens[r] - n + i.
+
+    Args:
+        q:            bf16 [T, H, 576] (512 absorbed latents, 64 rotated values)
+                      with the bf16 cache, [T, H, 512] with the INT8 cache
+        kv_cache:     bf16 [num_blocks, block_size, 576] (titan_kv.store_rope) or
+                      int8 [num_blocks, block_size, 528] (titan_kv.store_int8);
+                      row and page strides multiples of 16 bytes
+        cu_seqlens_q: int32 [R + 1], ascending from 0
+        seq_lens:     int32 [R], lengths with the new tokens
+        block_table:  int32 [R, max_blocks]; a position whose entry is outside
+                      [0, num_blocks) or past max_blocks is masked
+        sm_scale:     softmax scale
+        out:          bf16 [T, H, 512] to write to (allocated if None)
+        return_lse:   also return fp32 [T, H], the natural log of each sum
+
+    Returns out, or (out, lse).  A token that sees no position gets zeros and
+    -inf; rows of tokens at and past cu_seqlens_q[R] are not written.
+    """
+    if q.dim() != 3 or kv_cache.dim() != 3:
+        raise ValueError(f"q must be [T, H, D] and kv_cache [num_blocks, block_size, width], got {tuple(q.shape)}, "
+                         f"{tuple(kv_cache.shape)}")
+    int8 = kv_cache.dtype == torch.int8
+    width, dim = (_ROW_BYTES, _BLOCK_DMODEL) if int8 else (_DIM_QK, _DIM_QK)
+    if not int8 and kv_cache.dtype != torch.bfloat16:
+        raise ValueError(f"kv_cache must be bf16 or int8, got {kv_cache.dtype}")
+    if q.dtype != torch.bfloat16:
+        raise ValueError(f"q must be bf16, got {q.dtype}")
+    T, H, D = q.shape
+    if D != dim or kv_cache.shape[2] != width:
+        raise ValueError(f"a {kv_cache.dtype} cache has rows of {width} and queries of {dim}, got {kv_cache.shape[2]} "
+                         f"and {D}")
+    if H < 1 or kv_cache.shape[1] < 1:
+        raise ValueError("at least one head and one row per page")
+    if cu_seqlens_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.dtype != torch.int32:
+        raise ValueError("cu_seqlens_q, seq_lens and block_table must be int32")
+    R = seq_lens.numel()
+    if cu_seqlens_q.numel() != R + 1 or block_table.dim() != 2 or block_table.shape[0] != R:
+        raise ValueError(f"cu_seqlens_q must be [{R + 1}] and block_table [{R}, max_blocks] for seq_lens [{R}]")
+    dev = q.device
+    if not q.is_cuda or any(t.device != dev for t in (kv_cache, cu_seqlens_q, seq_lens, block_table)):
+        raise ValueError("mla_chunk_attention_paged requires CUDA (HIP) tensors on one device")
+    size = kv_cache.element_size()
+    page_bytes, row_bytes = kv_cache.stride(0) * size, kv_cache.stride(1) * size
+    if kv_cache.stride(2) != 1 or page_bytes % 16 or row_bytes % 16 or row_bytes < width * size \
+            or kv_cache.data_ptr() % 16:
+        raise ValueError("cache rows must be contiguous, 16-byte aligned, their strides multiples of 16 bytes")
+    if out is None:
+        out = torch.empty((T, H, _BLOCK_DV), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, H, _BLOCK_DV) or out.device != dev \
+            or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8:
+        raise ValueError(f"out must be bf16 [{T}, {H}, {_BLOCK_DV}] on q's device, rows contiguous and 8-byte aligned")
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    if T == 0 or R == 0:
+        return (out, lse) if return_lse else out
+    if q.stride(2) != 1 or q.stride(1) % 8 or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    cu_seqlens_q, seq_lens = cu_seqlens_q.contiguous(), seq_lens.contiguous()
+
+    L = _lib.load()
+    with torch.cuda.device(dev):
+        ws_bytes = L.glm53_chunk_mla_workspace_bytes(T, R, H)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+        rc = L.glm53_chunk_mla(
+            q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), int(int8), page_bytes, row_bytes,
+            kv_cache.shape[0], kv_cache.shape[1], cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
+            block_table.data_ptr(), R, block_table.stride(0), block_table.shape[1], T, H, float(sm_scale),
+            workspace.data_ptr() if workspace is not None else None, ws_bytes,
+            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if lse is not None else None,
+            _lib.stream_handle(dev))
+    _lib.check(rc, "glm53_chunk_mla")
+    return (out, lse) if return_lse else out
+
+
 def sparse_mla_partials(q, kv, indices, sm_scale, num_kv_splits):
     """First stage only: per-split normalised outputs and LSEs (fp32) in one
     buffer laid out as glm53.h documents (part [T*S*Hp, 512] then lse

@@ -432,6 +432,116 @@ int glm53_indexer_topk_next_n(const float* logits, int64_t sl,
 #define GLM53_PROBE_COPY_NT  2
 int glm53_stream_probe(int kind, const void* src, void* dst, int64_t bytes, void* stream);
 
+/*
+ * Dense causal latent attention of a chunk of new tokens over a paged cache
+ * (absorbed form).  No counterpart in the reference, whose attention reads
+ * indexed rows only; the rotary bf16 cache is the 576-wide form its attention
+ * names (kernels/titan_mla.py:17-56).
+ *
+ * Request r of num_reqs has the query tokens cu_seqlens_q[r] ..
+ * cu_seqlens_q[r + 1) - n of them - and seq_lens[r] cached positions, its own
+ * tokens the last n.  Its token i sees the positions j <= seq_lens[r] - n + i
+ * whose page block_table[r * bt_stride + j / block_size] lies in
+ * [0, num_blocks); positions past max_blocks * block_size are not seen.
+ *   out[t, h] = sum_j softmax_j(sm_scale * q[t, h] . k_j) * k_j[:512]
+ *   lse[t, h] = ln sum_j exp(sm_scale * q[t, h] . k_j)     (if lse is given)
+ * A token that sees nothing gets zeros and -inf.
+ *
+ *   q        bf16 [total_q, num_heads, 576 or 512], strides sq_t, sq_h
+ *            (elements, multiples of 8), 16-byte aligned, last dim contiguous.
+ *   kv_pages page 0; page b starts b * page_bytes later and holds block_size
+ *            rows row_bytes apart (multiples of 16).  kv_is_int8 = 0: bf16
+ *            rows of 512 latents and 64 rotary values (1152 bytes, q 576
+ *            wide); 1: the 528-byte INT8 rows of glm53_store_int8 (q 512).
+ *   cu_seqlens_q  int32 [num_reqs + 1], ascending.  Query tokens at and past
+ *            cu_seqlens_q[num_reqs] are padding: their out and lse rows are
+ *            left as they were.
+ *   workspace  glm53_chunk_mla_workspace_bytes(...) bytes, 16-byte aligned
+ *            (0: none needed).  Calls that may run at the same time, and
+ *            graphs that may, need one each.
+ *   out      bf16 [total_q, num_heads, 512], strides so_t, so_h (multiples of
+ *            4 elements, 8-byte aligned); lse fp32 [total_q, num_heads] or
+ *            NULL.
+ * total_q * num_heads + 64 * num_reqs must stay below 2^31.
+ */
+int64_t glm53_chunk_mla_workspace_bytes(int64_t total_q, int64_t num_reqs, int64_t num_heads);
+int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h,
+                    const void* kv_pages, int kv_is_int8, int64_t page_bytes, int64_t row_bytes,
+                    int64_t num_blocks, int64_t block_size,
+                    const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                    const int32_t* block_table, int64_t num_reqs, int64_t bt_stride,
+                    int64_t max_blocks, int64_t total_q, int64_t num_heads, double sm_scale,
+                    void* workspace, int64_t workspace_bytes,
+                    void* out, int64_t so_t, int64_t so_h, float* lse, void* stream);
+
+/*
+ * Appending to a paged bf16 latent cache with the position rotation on the
+ * way.  The reference has no writer for its 576-wide rows
+ * (kernels/titan_mla.py:17-56 names them); the rotation and the optional RMS
+ * norm are the steps that a rotary model takes before the row is stored.
+ *
+ * For token i < n_slots with position p = positions[i] and slot s = slots[i]:
+ * the row at cache + (s / block_size) * cache_stride_block
+ *               + (s % block_size) * cache_stride_slot  (bytes)
+ * receives 512 bf16 latents, x[i] or x[i] * norm_weight / sqrt(mean(x[i]^2) +
+ * eps) where norm_weight is given, then the 64 bf16 values of k_pe[i] rotated
+ * to p; and q_out[i, h] receives q_pe[i, h] rotated to p for num_heads heads.
+ * Rotation: the pair (a, b) of values k and k + 32 (interleaved: 2k and
+ * 2k + 1) becomes (a cos - b sin, b cos + a sin) with cos = cos_sin[p][k], sin
+ * = cos_sin[p][32 + k].  fp32 arithmetic, one rounding to bf16.
+ *
+ * A slot outside [0, capacity) is skipped (its queries are rotated); a
+ * position outside [0, max_pos) leaves the cache as it was and gives zero
+ * queries.  Slots of one call are distinct.  q_out may be q_pe.
+ * x, k_pe, q_pe, q_out: strides in elements; every base and stride a multiple
+ * of 16 bytes, cos_sin (fp32 or bf16 [max_pos][64]) and norm_weight (bf16
+ * [512] or NULL) contiguous and 16-byte aligned.
+ */
+int glm53_store_rope(const void* x, int64_t x_row_stride, const void* k_pe, int64_t k_row_stride,
+                     const void* positions, int positions_is_i64,
+                     const void* cos_sin, int cos_sin_is_f32, int64_t max_pos, int interleaved,
+                     const void* norm_weight, float eps,
+                     void* cache, int64_t cache_stride_block, int64_t cache_stride_slot,
+                     int64_t block_size, int64_t capacity,
+                     const void* slots, int slots_is_i64, int64_t n_slots,
+                     const void* q_pe, int64_t sq_t, int64_t sq_h,
+                     void* q_out, int64_t so_t, int64_t so_h, int64_t num_heads, void* stream);
+
+/*
+ * Drafted tokens against the target's probabilities, the end of a speculative
+ * decode step (no counterpart in the reference).
+ *
+ * Request r has the target rows cu_rows[r] .. cu_rows[r + 1) of target_probs
+ * (fp32 [num_rows][vocab], row stride st): one per draft, in order, and one
+ * more; its drafts are draft_ids[cu_rows[r] - r ...] with the draft model's
+ * rows draft_probs (fp32, row stride sd; NULL: drafts without probabilities).
+ * Draft x is taken while accept_u * q(x) < p(x) (fp32; q = 1 without
+ * draft_probs; an id outside [0, vocab) is not taken).  The first that is not
+ * is replaced by a token drawn from max(p - q, 0) (without draft_probs: from p
+ * without x); where all are taken one more is drawn from the last row's p.
+ * Token v weighs floor(min(max(., 0), 1) * 2^40), NaN 0; W is the weights' sum
+ * and the token the first whose running sum passes min(floor(sample_u[r] * W),
+ * W - 1).  Where W is 0 the row p itself serves; where that has no weight
+ * either the token is -1.
+ *
+ *   tokens    int32 [num_requests][max_drafts + 1]: the drafts taken, the
+ *             drawn token, then -1.  More than max_drafts drafts are not
+ *             looked at.
+ *   accepted  int32 [num_requests]: how many were taken.
+ *   workspace glm53_verify_drafts_workspace_bytes(...) bytes, 8-byte aligned;
+ *             calls that may run at the same time need one each.
+ * A request without rows, or whose rows lie outside the num_rows rows or
+ * num_drafts drafts, has only -1 and 0.  num_requests is at most 65535.
+ */
+int64_t glm53_verify_drafts_workspace_bytes(int64_t num_requests, int64_t vocab);
+int glm53_verify_drafts(const float* target_probs, int64_t st, int64_t num_rows,
+                        const float* draft_probs, int64_t sd,
+                        const void* draft_ids, int ids_is_i64, int64_t num_drafts,
+                        const int32_t* cu_rows, const float* accept_u, const double* sample_u,
+                        int64_t num_requests, int64_t vocab, int64_t max_drafts,
+                        void* workspace, int64_t workspace_bytes,
+                        int32_t* tokens, int32_t* accepted, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
