@@ -65,15 +65,10 @@ struct ChunkArgs {
   int2* shares;    // [num_tiles]: first and last workgroup of a shared tile, or -1
 };
 
-template <int kTM>
-struct ChunkShape {
-  static constexpr int kWaves = kTM == 64 ? 8 : 4;
-  static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kRowTiles = kTM / 16;
-  static constexpr int kRowGroups = kWaves / 4;          // QK: wave = row group x 16 keys
-  static constexpr int kRT = kRowTiles / kRowGroups;     // QK: row tiles of a wave
-  static constexpr int kLT = 32 / kWaves;                // PV: latent tiles of a wave
-};
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kOwn = kKeys / kWaves;      // keys of a block that a wave brings in, and takes in QK
+constexpr int kLT = 32 / kWaves;          // PV: latent tiles of a wave
 
 template <int kTM>
 struct __attribute__((aligned(16))) ChunkShared {
@@ -82,12 +77,12 @@ struct __attribute__((aligned(16))) ChunkShared {
     uint8_t rope[kKeys][2 * kRope];
   } kv[2];
   uint8_t p[kTM][kPPitch];             // P, keys of each 32 in the order of the V operand
-  float red[4][kTM];                   // per key group: block maximum, at the end the sum
+  float red[kWaves][kTM];              // per wave: its keys' maximum, at the end their sum
   float ref[kTM];                      // alpha when the reference moves, at the end the reference
   float scl[2][kKeys];                 // INT8 rows' scales
   int ends[kMaxSplitTiles];            // blocks up to and with each tile
   int reqs[kMaxSplitTiles];
-  int sums[8];
+  int sums[kWaves];
   int flag[2];
   int first;
 };
@@ -154,6 +149,37 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
   return w;
 }
 
+// One K-step's products of four row tiles, the queries in accumulation
+// registers (kAcc) or vector ones; with kFirst the sums start at 0.  In asm
+// because the compiler, with nearly all 512 registers of a lane in use, copies
+// the queries to vector registers before most products otherwise.  The two
+// wait states before the products are what a vector instruction that wrote
+// one of their operands needs; nothing but these products writes s, and
+// products_done() comes before its first other use.
+template <bool kFirst, bool kAcc>
+__device__ __forceinline__ void four_products(f32x4 (&s)[4], bf16x8 k, bf16x8 q0, bf16x8 q1, bf16x8 q2, bf16x8 q3) {
+  if constexpr (kFirst)
+    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, 0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, 0\n\t"
+        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, 0\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, 0"
+        : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+        : "v"(k), "a"(q0), "a"(q1), "a"(q2), "a"(q3));
+  else if constexpr (kAcc)
+    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, %1\n\t"
+        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, %3"
+        : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])
+        : "v"(k), "a"(q0), "a"(q1), "a"(q2), "a"(q3));
+  else
+    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, %1\n\t"
+        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, %3"
+        : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])
+        : "v"(k), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
+}
+// Wait states between a product and a vector instruction that reads it (11
+// for products of this shape; 16 here).
+__device__ __forceinline__ void products_done(f32x4 (&s)[4]) {
+  asm volatile("s_nop 15" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
+}
+
 // What a request's tokens and keys are, from values that may be anything:
 // token ranges are clipped to the queries there are, lengths to the table.
 struct Request {
@@ -184,19 +210,27 @@ __device__ __forceinline__ int last_key(const Request& r, int row0, int heads, i
   return k < 0 ? -1 : static_cast<int>(k < max_pos ? k : max_pos - 1);
 }
 
+// The kernel's arguments read where they are used, instead of being kept in
+// scalar registers from the start.
+__device__ __forceinline__ const ChunkArgs& late_args() {
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const ChunkArgs*)p;
+}
+
 template <int kTM, bool kInt8, bool kSplit>
-__global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(const ChunkArgs a) {
-  using Shape = ChunkShape<kTM>;
-  constexpr int kWaves = Shape::kWaves, kThreads = Shape::kThreads, kRowTiles = Shape::kRowTiles, kRT = Shape::kRT,
-                kLT = Shape::kLT;
-  constexpr int kPer = kKeys / kWaves;       // rows of a block that a wave brings in
+__global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
+  constexpr int kRT = kTM / 16;              // row tiles
   constexpr int kSteps = kInt8 ? 16 : 18;    // K-steps of 32
   __shared__ ChunkShared<kTM> sh;
 
   const int w = uniform(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int g = lane >> 4, c = lane & 15;
-  const int kg = w & 3, rg = w >> 2;
+  int lane = threadIdx.x & 63;
+  // What depends on the lane alone would be kept in registers across the
+  // block loop, which has none to spare: forget() makes the compiler derive it
+  // anew from the lane.
+  auto forget = [&]() { asm volatile("" : "+v"(lane)); };
+  int g = lane >> 4, c = lane & 15;
   const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.block_size;
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
@@ -242,6 +276,7 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
       if (i < w) before += s;
       total += s;
     }
+    total = uniform(total);
     if (total == 0) {
       if (blockIdx.x == 0)
         for (int t = threadIdx.x; t < a.num_tiles; t += kThreads) a.shares[t] = make_int2(-1, -1);
@@ -281,7 +316,6 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
       r = uniform(sh.reqs[tile]);
       b0 = max(lo - start, 0);
       b1 = min(hi - start, units);
-      rq = request_of(a.cu[r], a.cu[r + 1], a.lens[r], a.total_q);
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
       int count = 0;
@@ -295,9 +329,9 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
 #pragma unroll
       for (int i = 0; i < kWaves; i++) r += sh.sums[i];
       r = uniform(max(r, 0));
-      rq = request_of(a.cu[r], a.cu[r + 1], a.lens[r], a.total_q);
       b0 = b1 = units = 0;
     }
+    rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
@@ -310,163 +344,193 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
     // the least of the rows' last positions: keys past it are masked for some row
     const int64_t least64 = static_cast<int64_t>(rq.len) - rq.n + row0 / a.heads;
     const int least = static_cast<int>(least64 < -1 ? -1 : least64 < last ? least64 : last);
-    const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
 
-    // ---- the queries: row c of row tile rt of this wave's row group
-    bf16x8 qf[kRT][kSteps];
-    int limit[kRT];
-#pragma unroll
-    for (int rt = 0; rt < kRT; rt++) {
-      const int row = row0 + 16 * (rg * kRT + rt) + c;
-      const bool in = row < rows;
-      const int tok = in ? row / a.heads : 0, head = in ? row - tok * a.heads : 0;
-      const int64_t see = static_cast<int64_t>(rq.len) - rq.n + tok;
-      limit[rt] = in && see >= 0 ? static_cast<int>(see < last ? see : last) : -1;
-      const uint16_t* qr = a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t + static_cast<int64_t>(head) * a.sq_h + 8 * g;
-#pragma unroll
-      for (int s = 0; s < kSteps; s++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (in) v = *reinterpret_cast<const uint4*>(qr + 32 * s);
-        qf[rt][s] = __builtin_bit_cast(bf16x8, v);
+    if (kSplit) wg_barrier();   // the buffers are free (the tile before, the scan)
+
+    // ---- bringing blocks in.  Wave w brings in the 16 keys that it takes in
+    // QK.  Lane c (of each 16) looks up key 16 w + c: its page in the table,
+    // one block ahead of its use, then its row's address.  A key past the
+    // sequence, or whose page is not in the table or the cache, has none: the
+    // cache's first row is read in its place and zeroed.
+    uint2 codes[kInt8 ? kOwn : 1];
+    float scale = 0.f;
+    int pos = b0 * kKeys + kOwn * w + c;   // of the block that `page` is for
+    int pg = pos / a.block_size, in_page = pos - pg * a.block_size, page = -1;
+    const int step_pg = kKeys / a.block_size, step_in = kKeys - step_pg * a.block_size;
+    const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
+    auto look_up = [&](int b) { page = b < b1 && pos <= last && pg < a.max_blocks ? bt[pg] : -1; };
+    auto advance = [&]() {
+      pos += kKeys;
+      pg += step_pg;
+      in_page += step_in;
+      if (in_page >= a.block_size) in_page -= a.block_size, pg++;
+    };
+    uint32_t row_lo = 0, row_hi = 0, have = 0, have_next = 0;   // addresses; bit j: key 16 w + j has a row
+    auto address = [&]() {
+      const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
+      have_next = static_cast<uint32_t>(__ballot(ok)) & 0xffff;
+      const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
+                          (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
+      row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
+    };
+    // step j of kSteps of bringing in block b
+    auto bring = [&](int b, int j) {
+      auto& blk = sh.kv[b & 1];
+      if (j < kOwn) {
+        const uint64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, j)) |
+                            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, j))) << 32;
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(at);
+        if constexpr (kInt8)
+          codes[j] = *reinterpret_cast<const uint2*>(row + 8 * lane);
+        else
+          load_lds16(lds_offset(blk.lat[kOwn * w + j]), row, (16 * lane) ^ (16 * swizzle(j)));
+      } else if constexpr (!kInt8) {
+        const int key = 8 * (j - kOwn) + (lane >> 3);
+        const uint64_t at = static_cast<uint32_t>(__shfl(static_cast<int>(row_lo), key)) |
+                            static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row_hi), key))) << 32;
+        load_lds16_at(lds_offset(blk.rope[kOwn * w + 8 * (j - kOwn)]),
+                      reinterpret_cast<const uint8_t*>(at) + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(key)));
       }
+      if (kInt8 && j == kOwn - 1)
+        scale = *reinterpret_cast<const float*>((row_lo | static_cast<uint64_t>(row_hi) << 32) + kLatent);
+    };
+    // INT8: row j of the wave's keys of block b as bf16 into LDS (0 without a row)
+    auto put_row = [&](int b, int j) {
+      if constexpr (kInt8) {
+        const uint2 v = have_next >> j & 1 ? codes[j] : make_uint2(0, 0);
+        *reinterpret_cast<uint4*>(&sh.kv[b & 1].lat[kOwn * w + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
+        if (j == kOwn - 1 && lane < kOwn) sh.scl[b & 1][kOwn * w + lane] = have_next >> lane & 1 ? scale : 0.f;
+      }
+    };
+
+    if (b0 < b1) {
+      look_up(b0);
+      address();
+      advance();
+#pragma unroll
+      for (int j = 0; j < kSteps; j++) bring(b0, j);
+      look_up(b0 + 1);
     }
 
-    f32x4 acc[kLT][kRowTiles];
+    // ---- the queries: row c of row tile rt (rows past the last: the last, not stored)
+    bf16x8 qf[kRT][kSteps];
+#pragma unroll
+    for (int rt = 0; rt < kRT; rt++) {
+      const int row = min(row0 + 16 * rt + c, rows - 1);
+      const int tok = row / a.heads, head = row - tok * a.heads;
+      const uint16_t* qr = a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t + static_cast<int64_t>(head) * a.sq_h + 8 * g;
+#pragma unroll
+      for (int s = 0; s < kSteps; s++) qf[rt][s] = *reinterpret_cast<const bf16x8*>(qr + 32 * s);
+    }
+    f32x4 acc[kLT][kRT];
 #pragma unroll
     for (int i = 0; i < kLT; i++)
 #pragma unroll
-      for (int j = 0; j < kRowTiles; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < kRT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref[kRT], sum[kRT];
 #pragma unroll
     for (int rt = 0; rt < kRT; rt++) ref[rt] = -INFINITY, sum[rt] = 0.f;
-
-    // ---- bringing a block in.  Lane l looks up the row of key l: its byte
-    // offset in the cache, or none past the sequence or outside the table
-    // and the cache.
-    uint2 codes[kInt8 ? kPer : 1];
-    float scale = 0.f;
-    uint64_t valid = 0, valid_next = 0;   // bit k: key k of the block has a row
-    auto page_of = [&](int b) {           // the page of key `lane` of block b, -1: none
-      const int pos = b * kKeys + lane;
-      const int blk = pos / a.block_size;
-      return b < b1 && pos <= last && blk < a.max_blocks ? bt[blk] : -1;
-    };
-    auto issue = [&](int b, int page) {
-      const int pos = b * kKeys + lane;
-      const bool ok = page >= 0 && page < a.num_blocks;
-      valid_next = __ballot(ok);
-      const int64_t off =
-          ok ? page * a.page_bytes + static_cast<int64_t>(pos % a.block_size) * a.row_bytes : 0;
-      const int off_lo = static_cast<int>(off), off_hi = static_cast<int>(off >> 32);
-      auto& blk = sh.kv[b & 1];
-#pragma unroll
-      for (int j = 0; j < kPer; j++) {
-        const int key = w + kWaves * j;
-        const uint64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(off_lo, key)) |
-                            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(off_hi, key))) << 32;
-        const uint8_t* row = a.kv + at;
-        if constexpr (kInt8) {
-          codes[j] = make_uint2(0, 0);
-          if (valid_next >> key & 1) codes[j] = reinterpret_cast<const uint2*>(row)[lane];
-        } else if (valid_next >> key & 1) {
-          load_lds16(lds_offset(blk.lat[key]), row, 16 * (lane ^ swizzle(key)));
-        } else {
-          *reinterpret_cast<uint4*>(&blk.lat[key][16 * lane]) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if constexpr (kInt8) {
-        scale = 0.f;
-        if (w == 0 && ok) scale = *reinterpret_cast<const float*>(a.kv + off + kLatent);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kPer / 8; j++) {
-          const int k0 = 8 * (w + kWaves * j), key = k0 + (lane >> 3);
-          const uint64_t at = static_cast<uint32_t>(__shfl(off_lo, key)) |
-                              static_cast<uint64_t>(static_cast<uint32_t>(__shfl(off_hi, key))) << 32;
-          if (valid_next >> key & 1)
-            load_lds16_at(lds_offset(blk.rope[k0]), a.kv + at + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(key)));
-          else
-            *reinterpret_cast<uint4*>(&blk.rope[k0][16 * lane]) = make_uint4(0, 0, 0, 0);
-        }
-      }
-    };
-    auto store_codes = [&](int b) {   // INT8: the block's rows as bf16 into LDS
-      if constexpr (kInt8) {
-        auto& blk = sh.kv[b & 1];
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-          const int key = w + kWaves * j;
-          *reinterpret_cast<uint4*>(&blk.lat[key][16 * (lane ^ swizzle(key))]) = codes_to_bf16(codes[j]);
-        }
-        if (w == 0) sh.scl[b & 1][lane] = scale;
-      }
-    };
-
-    if (kSplit) wg_barrier();   // the buffers are free (the tile before, the scan)
-    int page = -1;
     if (b0 < b1) {
-      issue(b0, page_of(b0));
-      page = page_of(b0 + 1);
-      store_codes(b0);
+#pragma unroll
+      for (int j = 0; j < kOwn; j++) put_row(b0, j);
     }
     if (threadIdx.x == 0) sh.flag[0] = sh.flag[1] = 0;
 
     for (int b = b0; b < b1; b++) {
-      loads_done();
-      wg_barrier();   // block b is in LDS; nobody reads the other buffer, P or the maxima any more
-      valid = valid_next;
-      if (threadIdx.x == 0) sh.flag[(b + 1) & 1] = 0;
-      if (b + 1 < b1) {
-        issue(b + 1, page);
-        page = page_of(b + 2);
-      }
+      loads_done();   // this wave's rows of block b
+      wg_barrier();   // nobody reads the other buffer, P or the maxima any more
+      have = have_next;
       auto& blk = sh.kv[b & 1];
+      forget();
+      g = lane >> 4, c = lane & 15;
+      if (!kInt8 && have != 0xffff) {
+        for (int j = 0; j < kOwn; j++)
+          if (!(have >> j & 1)) {
+            *reinterpret_cast<uint4*>(&blk.lat[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
+            if (lane < 8) *reinterpret_cast<uint4*>(&blk.rope[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
+          }
+      }
+      if (w == 0 && lane == 0) sh.flag[(b + 1) & 1] = 0;
 
-      // ---- S^T = K Q^T: keys 16 kg + 4 g + i of the block, rows c
+      // ---- S^T = K Q^T: keys 16 w + 4 g + i of the block, rows c.  Each
+      // K-step's operand is read kAhead steps before its products, and between
+      // the steps a row of the next block is asked for.
       f32x4 s[kRT];
+      if constexpr (kRT != 4) {
 #pragma unroll
-      for (int rt = 0; rt < kRT; rt++) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rt = 0; rt < kRT; rt++) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      address();   // after the last block: no rows, the cache's first in their place
       {
-        const int key = 16 * kg + c, sw = swizzle(c);
-        const uint8_t* kr = blk.lat[key];
-        const uint8_t* even = kr + 16 * (g ^ sw);
-        const uint8_t* odd = kr + 16 * ((4 + g) ^ sw);
+        constexpr int kAhead = 3;
+        const int key = kOwn * w + c, sw = swizzle(c);
+        const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
+        const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
+        const uint8_t* rope = blk.rope[key];
+        auto operand = [&](int st) {
+          return *reinterpret_cast<const bf16x8*>(st < 16 ? (st & 1 ? odd : even) + 128 * (st >> 1)
+                                                          : rope + 16 * ((4 * (st - 16) + g) ^ sw));
+        };
+        bf16x8 k[kSteps];
 #pragma unroll
-        for (int st = 0; st < 16; st++) {
-          const bf16x8 k = *reinterpret_cast<const bf16x8*>((st & 1 ? odd : even) + 128 * (st >> 1));
+        for (int st = 0; st < kAhead; st++) k[st] = operand(st);
 #pragma unroll
-          for (int rt = 0; rt < kRT; rt++) s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[rt][st], s[rt], 0, 0, 0);
-        }
-        if constexpr (!kInt8) {
-#pragma unroll
-          for (int st = 0; st < 2; st++) {
-            const bf16x8 k = *reinterpret_cast<const bf16x8*>(&blk.rope[key][16 * ((4 * st + g) ^ sw)]);
+        for (int st = 0; st < kSteps; st++) {
+          if (st + kAhead < kSteps) k[st + kAhead] = operand(st + kAhead);
+          if constexpr (kRT == 4) {
+            if (st == 0)
+              four_products<true, true>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
+            else if (st < 16)
+              four_products<false, true>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
+            else
+              four_products<false, false>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
+          } else {
 #pragma unroll
             for (int rt = 0; rt < kRT; rt++)
-              s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[rt][16 + st], s[rt], 0, 0, 0);
+              s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], s[rt], 0, 0, 0);
+          }
+          bring(b + 1, st);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (kRT == 4) products_done(s);
+      }
+      advance();
+      look_up(b + 2);
+
+      forget();
+      g = lane >> 4, c = lane & 15;
+      const bool masked = (b + 1) * kKeys - 1 > least || have != 0xffff;   // uniform
+      float ksv[4] = {1.f, 1.f, 1.f, 1.f};
+      if constexpr (kInt8) {
+        const float4 ks = *reinterpret_cast<const float4*>(&sh.scl[b & 1][kOwn * w + 4 * g]);
+        ksv[0] = ks.x, ksv[1] = ks.y, ksv[2] = ks.z, ksv[3] = ks.w;
+      }
+#pragma unroll
+      for (int rt = 0; rt < kRT; rt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[rt][i] *= kInt8 ? a.scale_log2 * ksv[i] : a.scale_log2;
+      if (masked) {
+#pragma unroll
+        for (int rt = 0; rt < kRT; rt++) {
+          const int row = min(row0 + 16 * rt + c, rows - 1);
+          const int64_t see = static_cast<int64_t>(rq.len) - rq.n + row / a.heads;
+          const int limit = static_cast<int>(see < last ? see < -1 ? -1 : see : last) - b * kKeys;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int k = 4 * g + i;
+            if (kOwn * w + k > limit || !(have >> k & 1)) s[rt][i] = -INFINITY;
           }
         }
       }
-      const bool masked = (b + 1) * kKeys - 1 > least || valid != ~0ull;   // uniform
-      float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
-      if constexpr (kInt8) ks = *reinterpret_cast<const float4*>(&sh.scl[b & 1][16 * kg + 4 * g]);
-      const float ksv[4] = {ks.x, ks.y, ks.z, ks.w};
-      float top[kRT];
+      float top[kRT], mine = 0.f;
       bool moved = false;
 #pragma unroll
       for (int rt = 0; rt < kRT; rt++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          s[rt][i] *= kInt8 ? a.scale_log2 * ksv[i] : a.scale_log2;
-          if (masked) {
-            const int k = 16 * kg + 4 * g + i;
-            if (b * kKeys + k > limit[rt] || !(valid >> k & 1)) s[rt][i] = -INFINITY;
-          }
-        }
         top[rt] = quad_max(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3])));
         moved |= top[rt] > ref[rt] + kSlack;
-        if (g == 0) sh.red[kg][16 * (rg * kRT + rt) + c] = top[rt];
+        if (g == rt) mine = top[rt];
       }
+      if (lane < kTM) sh.red[w][lane] = mine;   // row 16 g + c
       if (__ballot(moved) && lane == 0) sh.flag[b & 1] = 1;
 
       // P of this wave's keys, against the reference (0 where a row has seen nothing)
@@ -482,39 +546,34 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
           if constexpr (kInt8) {
             // V = codes * scale: the scale goes to P, which a masked key has as 0 whatever its scale is
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = masked && s[rt][i] == -INFINITY ? 0.f : p[i] * ksv[i];
+            for (int i = 0; i < 4; i++) p[i] = s[rt][i] == -INFINITY ? 0.f : p[i] * ksv[i];
           }
-          // P is rounded to bf16 (2^-9 of each weight, no more than the
+          // P is rounded to bf16 (2^-9 of each weight on the average, like the
           // output's own rounding); the sum keeps the unrounded weights
-          uint2 v = make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
-          *reinterpret_cast<uint2*>(&sh.p[16 * (rg * kRT + rt) + c][64 * (kg >> 1) + 16 * g + 8 * (kg & 1)]) = v;
+          *reinterpret_cast<uint2*>(&sh.p[16 * rt + c][64 * (w >> 1) + 16 * g + 8 * (w & 1)]) =
+              make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
         }
       };
       put_p();
-      wg_barrier();   // P is whole, the block's keys have been read
+      wg_barrier();   // P is whole; every wave's rows are there
 
       if (uniform(sh.flag[b & 1])) {   // some row's maximum passed its reference: all rows take theirs
 #pragma unroll
         for (int rt = 0; rt < kRT; rt++) {
-          const int row = 16 * (rg * kRT + rt) + c;
+          const int row = 16 * rt + c;
           float m = ref[rt];
 #pragma unroll
-          for (int i = 0; i < 4; i++) m = fmaxf(m, sh.red[i][row]);
+          for (int i = 0; i < kWaves; i++) m = fmaxf(m, sh.red[i][row]);
           const float alpha = __builtin_amdgcn_exp2f(ref[rt] - (m == -INFINITY ? 0.f : m));
           ref[rt] = m;
           sum[rt] *= alpha;
-          if (kg == 0 && g == 0) sh.ref[row] = alpha;
-        }
-        put_p();
-        wg_barrier();
-#pragma unroll
-        for (int j = 0; j < kRowTiles; j++) {
-          const float alpha = sh.ref[16 * j + c];
 #pragma unroll
           for (int i = 0; i < kLT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[i][j][e] *= alpha;
+            for (int e = 0; e < 4; e++) acc[i][rt][e] *= alpha;
         }
+        put_p();
+        wg_barrier();
       }
 #pragma unroll
       for (int rt = 0; rt < kRT; rt++) sum[rt] += part[rt];
@@ -523,90 +582,106 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads) void chunk_mla_kernel(co
         // Keys that some row of the tile may not see: 0 * inf would put NaN
         // into that row.  A row that sees such a key has NaN from its logit.
         if ((b + 1) * kKeys - 1 > least && least < last) {
-          for (int key = w; key < kKeys; key += kWaves) {
-            uint4* at = reinterpret_cast<uint4*>(&blk.lat[key][16 * lane]);
-            uint4 v = *at;
-            v = make_uint4(finite_bf16x2(v.x), finite_bf16x2(v.y), finite_bf16x2(v.z), finite_bf16x2(v.w));
-            *at = v;
+          for (int j = 0; j < kOwn; j++) {
+            uint4* at = reinterpret_cast<uint4*>(&blk.lat[kOwn * w + j][16 * lane]);
+            const uint4 v = *at;
+            *at = make_uint4(finite_bf16x2(v.x), finite_bf16x2(v.y), finite_bf16x2(v.z), finite_bf16x2(v.w));
           }
           wg_barrier();
         }
       }
 
-      // ---- O^T += V^T P^T: latents 16 (kLT w + i) + 4 g + e, rows 16 j + c
-      const int tr_row = 4 * g + (c >> 2), tr_sw = swizzle(tr_row);
+      forget();
+      g = lane >> 4, c = lane & 15;
+      // ---- O^T += V^T P^T: latents 16 (kLT w + i) + 4 g + e, rows 16 j + c;
+      // V's operands two steps ahead.  INT8: a row of the next block is
+      // converted between the steps.
+      {
+        constexpr int kPv = 2 * kLT, kAhead = 2;
+        const int tr_row = 4 * g + (c >> 2), tr_sw = swizzle(tr_row);
+        const uint8_t* vr[4];
 #pragma unroll
-      for (int ks2 = 0; ks2 < 2; ks2++) {
-        bf16x8 pb[kRowTiles];
-#pragma unroll
-        for (int j = 0; j < kRowTiles; j++)
-          pb[j] = *reinterpret_cast<const bf16x8*>(&sh.p[16 * j + c][64 * ks2 + 16 * g]);
-#pragma unroll
-        for (int i = 0; i < kLT; i++) {
-          const int lt = kLT * w + i;
-          const int col = 128 * (lt >> 2) + 16 * ((2 * (lt & 3) + ((c & 3) >> 1)) ^ tr_sw) + 8 * (c & 1);
-          const uint8_t* vr = &blk.lat[32 * ks2 + tr_row][col];
-          const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, vr)));
+        for (int i = 0; i < 4; i++)
+          vr[i] = &blk.lat[tr_row][256 * w + 16 * ((2 * i + ((c & 3) >> 1)) ^ tr_sw) + 8 * (c & 1)];
+        auto operand = [&](int u) {
+          const uint8_t* p = vr[u & 3] + 128 * (u >> 2 & 1) + 32 * 2 * kLatent * (u >> 3);
+          const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p)));
           const i32x2 v1 = __builtin_bit_cast(
-              i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, vr + 16 * 2 * kLatent)));
-          const bf16x8 v = __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
+              i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p + 16 * 2 * kLatent)));
+          return __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
+        };
+        bf16x8 pb[2][kRT], v[kPv];
 #pragma unroll
-          for (int j = 0; j < kRowTiles; j++)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < kRT; j++) pb[0][j] = *reinterpret_cast<const bf16x8*>(&sh.p[16 * j + c][16 * g]);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) v[u] = operand(u);
+#pragma unroll
+        for (int u = 0; u < kPv; u++) {
+          if (u + kAhead < kPv) v[u + kAhead] = operand(u + kAhead);
+          if (u >= kLT - kRT && u < kLT) {
+            const int j = u - (kLT - kRT);
+            pb[1][j] = *reinterpret_cast<const bf16x8*>(&sh.p[16 * j + c][64 + 16 * g]);
+          }
+#pragma unroll
+          for (int j = 0; j < kRT; j++)
+            acc[u % kLT][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[u / kLT][j], acc[u % kLT][j], 0, 0, 0);
+          put_row(b + 1, u);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (b + 1 < b1) store_codes(b + 1);
     }
+    loads_done();   // what the last block asked for
 
     // ---- the rows' sums and references, then the output or the partial
     wg_barrier();
 #pragma unroll
     for (int rt = 0; rt < kRT; rt++) {
-      const int row = 16 * (rg * kRT + rt) + c;
       const float l = quad_sum(sum[rt]);
-      if (g == 0) sh.red[kg][row] = l;
-      if (kg == 0 && g == 0) sh.ref[row] = ref[rt];
+      if (g == 0) sh.red[w][16 * rt + c] = l;
+      if (w == 0 && g == 0) sh.ref[16 * rt + c] = ref[rt];
     }
     wg_barrier();
-    const bool whole = !kSplit || (lo <= start && start + units <= hi);
-    if (whole) {
+    const ChunkArgs& e = late_args();
+    if (!kSplit || (lo <= start && start + units <= hi)) {
 #pragma unroll
-      for (int j = 0; j < kRowTiles; j++) {
+      for (int j = 0; j < kRT; j++) {
         const int row = row0 + 16 * j + c;
         if (row < rows) {
           const float l = (sh.red[0][16 * j + c] + sh.red[1][16 * j + c]) + (sh.red[2][16 * j + c] + sh.red[3][16 * j + c]);
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int tok = row / a.heads, head = row - tok * a.heads;
-          uint16_t* o = a.out + static_cast<int64_t>(rq.t0 + tok) * a.so_t + static_cast<int64_t>(head) * a.so_h;
+          const int tok = row / e.heads, head = row - tok * e.heads;
+          uint16_t* o = e.out + static_cast<int64_t>(rq.t0 + tok) * e.so_t + static_cast<int64_t>(head) * e.so_h;
 #pragma unroll
           for (int i = 0; i < kLT; i++) {
             const f32x4 v = acc[i][j];
             *reinterpret_cast<uint2*>(o + 16 * (kLT * w + i) + 4 * g) =
                 make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
           }
-          if (a.lse && w == 0 && g == 0)
-            a.lse[static_cast<int64_t>(rq.t0 + tok) * a.heads + head] =
+          if (e.lse && w == 0 && g == 0)
+            e.lse[static_cast<int64_t>(rq.t0 + tok) * e.heads + head] =
                 l == 0.f ? -INFINITY : (sh.ref[16 * j + c] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
-      if (kSplit && threadIdx.x == 0) a.shares[tile] = make_int2(-1, -1);
+      if (kSplit && threadIdx.x == 0) e.shares[tile] = make_int2(-1, -1);
     } else {
       // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins here
       const int slot = 2 * static_cast<int>(blockIdx.x) + (lo <= start);
-      float* part = a.part + static_cast<int64_t>(slot) * (kTM * kLatent);
+      float* part = e.part + static_cast<int64_t>(slot) * (kTM * kLatent);
 #pragma unroll
       for (int i = 0; i < kLT; i++)
 #pragma unroll
-        for (int j = 0; j < kRowTiles; j++)
-          *reinterpret_cast<f32x4*>(part + ((kLT * w + i) * kRowTiles + j) * 256 + 4 * lane) = acc[i][j];
-      for (int row = threadIdx.x; row < kTM; row += kThreads)
-        a.ml[static_cast<int64_t>(slot) * kTM + row] =
+        for (int j = 0; j < kRT; j++)
+          *reinterpret_cast<f32x4*>(part + ((kLT * w + i) * kRT + j) * 256 + 4 * lane) = acc[i][j];
+      if (threadIdx.x < kTM) {
+        const int row = threadIdx.x;
+        e.ml[static_cast<int64_t>(slot) * kTM + row] =
             make_float2(sh.ref[row], (sh.red[0][row] + sh.red[1][row]) + (sh.red[2][row] + sh.red[3][row]));
+      }
       if (lo <= start && threadIdx.x == 0) {
         const int64_t groups = min(static_cast<int>(gridDim.x), total);
         // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
         const int64_t last_unit = start + units;
-        a.shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
+        e.shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
       }
     }
     if (!kSplit) return;
@@ -725,14 +800,14 @@ Workspace workspace_of(int tm, int64_t tiles) {
 template <int kTM, bool kInt8>
 int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
   if (a.num_tiles > kMaxSplitTiles) {
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM>), dim3(32 * kTM / 16, a.num_tiles), dim3(64 * kMergeWaves), 0, st, a);
   }
   return static_cast<int>(hipGetLastError());
