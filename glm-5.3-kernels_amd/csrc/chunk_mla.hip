@@ -59,6 +59,7 @@ struct ChunkArgs {
   float scale_log2;
   uint16_t* out;
   int64_t so_t, so_h;
+  int out_align16; // out rows 16-byte aligned (else 8)
   float* lse;      // [total_q][heads], or null
   float* part;     // [2 * workgroups] slots of kTM x 512, accumulator order
   float2* ml;      // [2 * workgroups][kTM]: reference maximum (log2) and sum
@@ -373,7 +374,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
                           (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
       row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
     };
-    // step j of kSteps of bringing in block b
+    // Step j of kSteps of bringing in block b.  With 64 rows the products
+    // bound the loop, and the loads are spread over it: sent at once they
+    // fill the CU's miss queue and hold up the products behind them.
+    constexpr bool kSpread = kRT == 4 && !kInt8;
     auto bring = [&](int b, int j) {
       auto& blk = sh.kv[b & 1];
       if (j < kOwn) {
@@ -412,15 +416,43 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       look_up(b0 + 1);
     }
 
-    // ---- the queries: row c of row tile rt (rows past the last: the last, not stored)
+    // ---- the queries: row c of row tile rt (rows past the last: the last,
+    // not stored).  Every wave needs all of them, so they come through LDS
+    // once, in the buffer that the second block will take, laid out like keys:
+    // wave w brings in every fourth row.
     bf16x8 qf[kRT][kSteps];
-#pragma unroll
-    for (int rt = 0; rt < kRT; rt++) {
-      const int row = min(row0 + 16 * rt + c, rows - 1);
+    {
+      auto& qs = sh.kv[(b0 + 1) & 1];
+      constexpr int kMine = kTM / kWaves;
+      const int row = min(row0 + kWaves * min(c, kMine - 1) + w, rows - 1);
       const int tok = row / a.heads, head = row - tok * a.heads;
-      const uint16_t* qr = a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t + static_cast<int64_t>(head) * a.sq_h + 8 * g;
+      const uint64_t at = reinterpret_cast<uint64_t>(a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t +
+                                                     static_cast<int64_t>(head) * a.sq_h);
+      const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
 #pragma unroll
-      for (int s = 0; s < kSteps; s++) qf[rt][s] = *reinterpret_cast<const bf16x8*>(qr + 32 * s);
+      for (int j = 0; j < kMine; j++) {
+        const uint64_t from = static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, j)) |
+                              static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, j))) << 32;
+        const int key = kWaves * j + w;
+        load_lds16(lds_offset(qs.lat[key]), reinterpret_cast<const uint8_t*>(from), 16 * (lane ^ swizzle(key)));
+        if constexpr (!kInt8) {
+          if (lane < 8)
+            load_lds16(lds_offset(qs.rope[key]), reinterpret_cast<const uint8_t*>(from),
+                       2 * kLatent + 16 * (lane ^ swizzle(key)));
+        }
+      }
+      loads_done();   // the queries, and the first block's rows
+      wg_barrier();
+#pragma unroll
+      for (int rt = 0; rt < kRT; rt++) {
+        const int key = 16 * rt + c, sw = swizzle(c);
+#pragma unroll
+        for (int st = 0; st < kSteps; st++) {
+          const uint8_t* from = st < 16 ? qs.lat[key] + 16 * ((4 * (st & 1) + g) ^ sw) + 128 * (st >> 1)
+                                        : qs.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
+          qf[rt][st] = *reinterpret_cast<const bf16x8*>(from);
+        }
+      }
     }
     f32x4 acc[kLT][kRT];
 #pragma unroll
@@ -462,7 +494,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       }
       address();   // after the last block: no rows, the cache's first in their place
       {
-        constexpr int kAhead = 3;
+        constexpr int kAhead = 5;
         const int key = kOwn * w + c, sw = swizzle(c);
         const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
         const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
@@ -489,13 +521,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             for (int rt = 0; rt < kRT; rt++)
               s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], s[rt], 0, 0, 0);
           }
-          bring(b + 1, st);
+          if (!kSpread || st % 2 == 0) bring(b + 1, kSpread ? st / 2 : st);
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (kRT == 4) products_done(s);
       }
-      advance();
-      look_up(b + 2);
+      if (kSpread) bring(b + 1, 9), bring(b + 1, 10);
 
       forget();
       g = lane >> 4, c = lane & 15;
@@ -555,6 +586,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         }
       };
       put_p();
+      if (kSpread) bring(b + 1, 11), bring(b + 1, 12);
+      advance();
+      look_up(b + 2);
       wg_barrier();   // P is whole; every wave's rows are there
 
       if (uniform(sh.flag[b & 1])) {   // some row's maximum passed its reference: all rows take theirs
@@ -597,7 +631,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       // V's operands two steps ahead.  INT8: a row of the next block is
       // converted between the steps.
       {
-        constexpr int kPv = 2 * kLT, kAhead = 2;
+        constexpr int kPv = 2 * kLT, kAhead = 3;
         const int tr_row = 4 * g + (c >> 2), tr_sw = swizzle(tr_row);
         const uint8_t* vr[4];
 #pragma unroll
@@ -625,6 +659,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
           for (int j = 0; j < kRT; j++)
             acc[u % kLT][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[u / kLT][j], acc[u % kLT][j], 0, 0, 0);
+          if (kSpread && u < 5) bring(b + 1, 13 + u);
           put_row(b + 1, u);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -643,23 +678,36 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     wg_barrier();
     const ChunkArgs& e = late_args();
     if (!kSplit || (lo <= start && start + units <= hi)) {
+      // whole rows go out: the row tiles as bf16 through LDS (8 bytes of row
+      // c at 16-byte chunk ^ (c % 8), so that rows fall on different banks),
+      // then each wave stores every fourth row
+      uint8_t(*os)[2 * kLatent] = sh.kv[0].lat;
 #pragma unroll
       for (int j = 0; j < kRT; j++) {
-        const int row = row0 + 16 * j + c;
-        if (row < rows) {
-          const float l = (sh.red[0][16 * j + c] + sh.red[1][16 * j + c]) + (sh.red[2][16 * j + c] + sh.red[3][16 * j + c]);
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int tok = row / e.heads, head = row - tok * e.heads;
-          uint16_t* o = e.out + static_cast<int64_t>(rq.t0 + tok) * e.so_t + static_cast<int64_t>(head) * e.so_h;
+        const float l = (sh.red[0][16 * j + c] + sh.red[1][16 * j + c]) + (sh.red[2][16 * j + c] + sh.red[3][16 * j + c]);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-          for (int i = 0; i < kLT; i++) {
-            const f32x4 v = acc[i][j];
-            *reinterpret_cast<uint2*>(o + 16 * (kLT * w + i) + 4 * g) =
-                make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
-          }
-          if (e.lse && w == 0 && g == 0)
-            e.lse[static_cast<int64_t>(rq.t0 + tok) * e.heads + head] =
-                l == 0.f ? -INFINITY : (sh.ref[16 * j + c] + __builtin_amdgcn_logf(l)) * kLn2;
+        for (int i = 0; i < kLT; i++) {
+          const f32x4 v = acc[i][j];
+          *reinterpret_cast<uint2*>(&os[16 * j + c][((32 * (kLT * w + i) + 16 * (g >> 1)) ^ (16 * (c & 7))) + 8 * (g & 1)]) =
+              make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+        }
+      }
+      wg_barrier();
+      for (int j = w; j < kTM && row0 + j < rows; j += kWaves) {
+        const int row = row0 + j, tok = row / e.heads, head = row - tok * e.heads;
+        uint16_t* o = e.out + static_cast<int64_t>(rq.t0 + tok) * e.so_t + static_cast<int64_t>(head) * e.so_h;
+        const uint4 v = *reinterpret_cast<const uint4*>(&os[j][(16 * lane) ^ (16 * (j & 7))]);
+        if (e.out_align16) {
+          reinterpret_cast<uint4*>(o)[lane] = v;
+        } else {
+          reinterpret_cast<uint2*>(o)[2 * lane] = make_uint2(v.x, v.y);
+          reinterpret_cast<uint2*>(o)[2 * lane + 1] = make_uint2(v.z, v.w);
+        }
+        if (e.lse && lane == 0) {
+          const float l = (sh.red[0][j] + sh.red[1][j]) + (sh.red[2][j] + sh.red[3][j]);
+          e.lse[static_cast<int64_t>(rq.t0 + tok) * e.heads + head] =
+              l == 0.f ? -INFINITY : (sh.ref[j] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
       if (kSplit && threadIdx.x == 0) e.shares[tile] = make_int2(-1, -1);
@@ -688,45 +736,45 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   }
 }
 
-constexpr int kMergeWaves = 8;
-
-// Joins a shared tile's partials: one workgroup per 16 rows x 16 latents, its
-// waves taking every eighth partial each, then joining theirs through LDS.
-template <int kTM>
-__global__ __launch_bounds__(64 * kMergeWaves) void chunk_mla_merge_kernel(const ChunkArgs a) {
-  constexpr int kRowTiles = kTM / 16;
-  __shared__ float acc_s[kMergeWaves][64][4];
-  __shared__ float2 ml_s[kMergeWaves][16];
+// Joins a shared tile's partials, 16 rows x 16 latents a job.  kTogether
+// waves take every kTogether-th partial each and join theirs through LDS (few
+// tiles, whose partials are many), or each of a workgroup's four waves takes a
+// job of its own.  kDeep partials are asked for at once.
+template <int kTM, int kTogether>
+__global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(const ChunkArgs a) {
+  constexpr int kRT = kTM / 16, kDeep = 8;
+  __shared__ float acc_s[kTogether][64][4];
+  __shared__ float2 ml_s[kTogether][16];
   const int tile = blockIdx.y;
   const int2 share = a.shares[tile];
   if (share.x < 0) return;
   const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int j = blockIdx.x % kRowTiles, lt = blockIdx.x / kRowTiles;
+  const int job = kTogether > 1 ? blockIdx.x : 4 * blockIdx.x + w;
+  const int j = job % kRT, lt = job / kRT;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  constexpr int kDeep = 4;
-  for (int k0 = share.x + w; k0 <= share.y; k0 += kMergeWaves * kDeep) {
+  for (int k0 = share.x + (kTogether > 1 ? w : 0); k0 <= share.y; k0 += kTogether * kDeep) {
     float2 ml[kDeep];
     f32x4 v[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; d++) {
-      const int k = k0 + kMergeWaves * d;
-      ml[d] = make_float2(-INFINITY, 0.f);
-      v[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (k <= share.y) {
-        const int64_t slot = 2 * static_cast<int64_t>(k) + (k == share.x);
-        ml[d] = a.ml[slot * kTM + 16 * j + c];
-        v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + (lt * kRowTiles + j) * 256 + 4 * lane);
-      }
+      const int k = min(k0 + kTogether * d, share.y);
+      const int64_t slot = 2 * static_cast<int64_t>(k) + (k == share.x);
+      ml[d] = a.ml[slot * kTM + 16 * j + c];
+      v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + (lt * kRT + j) * 256 + 4 * lane);
     }
     float top = m;
 #pragma unroll
-    for (int d = 0; d < kDeep; d++) top = fmaxf(top, ml[d].x);
+    for (int d = 0; d < kDeep; d++) {
+      if (k0 + kTogether * d > share.y) ml[d] = make_float2(-INFINITY, 0.f), v[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+      top = fmaxf(top, ml[d].x);
+    }
     const float base = top == -INFINITY ? 0.f : top;
     const float old = __builtin_amdgcn_exp2f(m - base);
     m = top;
     l *= old;
-    acc *= old;
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] *= old;
 #pragma unroll
     for (int d = 0; d < kDeep; d++) {
       const float f = __builtin_amdgcn_exp2f(ml[d].x - base);
@@ -735,24 +783,27 @@ __global__ __launch_bounds__(64 * kMergeWaves) void chunk_mla_merge_kernel(const
       for (int e = 0; e < 4; e++) acc[e] += f * v[d][e];
     }
   }
-  *reinterpret_cast<f32x4*>(acc_s[w][lane]) = acc;
-  if (g == 0) ml_s[w][c] = make_float2(m, l);
-  __syncthreads();
-  if (w) return;
-  float top = -INFINITY;
+  if constexpr (kTogether > 1) {
+    *reinterpret_cast<f32x4*>(acc_s[w][lane]) = acc;
+    if (g == 0) ml_s[w][c] = make_float2(m, l);
+    __syncthreads();
+    if (w) return;
+    float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kMergeWaves; i++) top = fmaxf(top, ml_s[i][c].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  l = 0.f;
-  acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kTogether; i++) top = fmaxf(top, ml_s[i][c].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    m = top;
+    l = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kMergeWaves; i++) {
-    const float2 ml = ml_s[i][c];
-    const float f = __builtin_amdgcn_exp2f(ml.x - base);
-    l += f * ml.y;
-    const f32x4 v = *reinterpret_cast<const f32x4*>(acc_s[i][lane]);
+    for (int i = 0; i < kTogether; i++) {
+      const float2 ml = ml_s[i][c];
+      const float f = __builtin_amdgcn_exp2f(ml.x - base);
+      l += f * ml.y;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(acc_s[i][lane]);
 #pragma unroll
-    for (int e = 0; e < 4; e++) acc[e] += f * v[e];
+      for (int e = 0; e < 4; e++) acc[e] += f * v[e];
+    }
   }
   // the request of the tile
   int at = 0;
@@ -770,7 +821,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void chunk_mla_merge_kernel(const
       make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   if (a.lse && lt == 0 && g == 0)
     a.lse[static_cast<int64_t>(rq.t0 + tok) * a.heads + head] =
-        l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Rows per tile: as many as a request's rows fill, 16, 32 or 64.
@@ -808,7 +859,12 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
     hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM>), dim3(32 * kTM / 16, a.num_tiles), dim3(64 * kMergeWaves), 0, st, a);
+    // a shared tile has about CUs / tiles partials: 16 waves on a job where
+    // that is many, one where it is few
+    if (a.num_tiles <= 16)
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 16>), dim3(2 * kTM, a.num_tiles), dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 1>), dim3(kTM / 2, a.num_tiles), dim3(256), 0, st, a);
   }
   return static_cast<int>(hipGetLastError());
 }
@@ -869,6 +925,7 @@ extern "C" int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h, const 
   a.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
   a.out = static_cast<uint16_t*>(out);
   a.so_t = so_t, a.so_h = so_h;
+  a.out_align16 = oa % 16 == 0 && so_t % 8 == 0 && so_h % 8 == 0;
   a.lse = lse;
   if (kv_is_int8) {
     if (tm == 16) return launch<16, true>(a, workspace, st);
