@@ -10,23 +10,33 @@
 // rotary values, or the 528-byte INT8 rows (512 codes and their scale).
 //
 // Work: the (token, head) rows of a request are flattened and cut into tiles
-// of kTM rows, which share every key they read; a tile walks its keys in
-// blocks of 64.  One workgroup (4 waves for 16 or 32 rows, 8 for 64):
-//   * a block's rows come into LDS (bf16 rows by direct global -> LDS loads,
-//     INT8 rows through registers, converted once), two buffers, the next
-//     block's loads in flight while this one is used;
-//   * S^T = K Q^T: each wave takes 16 of the 64 keys (and half of the rows
-//     where there are 64), its queries held in registers for the whole tile;
+// of kTM rows (16, 32 or 64), which share every key they read; a tile walks
+// its keys in blocks of 64.  Per block, of one workgroup:
+//   * the block's rows come into LDS (bf16 rows by direct global -> LDS loads,
+//     INT8 rows converted to bf16 once), two buffers, the next block's loads
+//     on their way while this one is used;
+//   * S^T = K Q^T, the queries held in registers for the whole tile;
 //   * softmax against a reference maximum that moves only when some row's
-//     maximum passes it by 2^8 (the sums and products scale with it, in fp32),
-//     so most blocks need one barrier between the two products;
-//   * O^T += V^T P^T: each wave takes its slice of the 512 latents for all
-//     rows; P goes through LDS as bf16, V is read from the same rows with
-//     transposing reads.
+//     maximum passes it by 2^8 (sums and output are scaled to it in fp32), so
+//     that most blocks need no exchange of maxima between the two products;
+//   * O^T += V^T P^T, each wave its slice of the 512 latents for all rows: P
+//     goes through LDS as bf16, V is read from the same rows with transposing
+//     reads.
+// 64 rows are bound by the products.  Four waves, one per SIMD, so that a lane
+// has 512 registers (queries 144, output 128); products of 32 x 32 x 16, which
+// need half the instructions and operand reads of the small ones - a single
+// wave issues about one instruction in 4 to 5 cycles, and that, not the matrix
+// cores, was the limit with 16 x 16 x 32 (6600 cycles a block).  A wave takes
+// 32 keys x 32 rows in QK and 128 latents x 64 rows in PV.
+// 16 and 32 rows are bound by memory.  Eight waves and products of 16 x 16 x
+// 32: a wave takes 16 keys x 16 rows in QK (of a 16-row tile four waves take
+// none) and 64 latents in PV.
 // Few tiles (decode): the blocks of all tiles are laid end to end and cut
 // into equal runs, one per workgroup; a tile that several workgroups share
 // leaves fp32 partials that the merge kernel joins.  Many tiles: one
 // workgroup each, longest first.
+#include <type_traits>
+
 #include "glm53_common.h"
 
 namespace glm53 {
@@ -36,7 +46,6 @@ constexpr int kLatent = 512;
 constexpr int kRope = 64;
 constexpr int kKeys = 64;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
-constexpr int kPPitch = 2 * kKeys + 16;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;       // how far (log2) a row's maximum may pass the reference
 
@@ -53,6 +62,7 @@ struct ChunkArgs {
   int max_blocks;
   int block_size;
   int num_reqs;
+  int first_step;  // of a binary search over the requests: the largest power of two below num_reqs, or 0
   int total_q;
   int heads;
   int num_tiles;   // bound: tile indexes are below it
@@ -66,10 +76,15 @@ struct ChunkArgs {
   int2* shares;    // [num_tiles]: first and last workgroup of a shared tile, or -1
 };
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kOwn = kKeys / kWaves;      // keys of a block that a wave brings in, and takes in QK
-constexpr int kLT = 32 / kWaves;          // PV: latent tiles of a wave
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+
+template <int kTM>
+struct ChunkShape {
+  static constexpr bool kBig = kTM == 64;           // products of 32 x 32 x 16
+  static constexpr int kWaves = kBig ? 4 : 8;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kOwn = kKeys / kWaves;       // rows of a block that a wave brings in
+};
 
 template <int kTM>
 struct __attribute__((aligned(16))) ChunkShared {
@@ -77,14 +92,15 @@ struct __attribute__((aligned(16))) ChunkShared {
     uint8_t lat[kKeys][2 * kLatent];   // chunk c of 16 bytes of row k at chunk c ^ swizzle(k)
     uint8_t rope[kKeys][2 * kRope];
   } kv[2];
-  uint8_t p[kTM][kPPitch];             // P, keys of each 32 in the order of the V operand
-  float red[kWaves][kTM];              // per wave: its keys' maximum, at the end their sum
+  uint8_t p[kTM][2 * kKeys];           // P, chunk c of row r at c ^ (r % 8), keys in the order of the V operand
+  float red[4][kTM];                   // per key group: maxima; at the end the sums
   float ref[kTM];                      // alpha when the reference moves, at the end the reference
   float scl[2][kKeys];                 // INT8 rows' scales
+  uint64_t have[2];                    // bit k: key k of the block has a row
   int ends[kMaxSplitTiles];            // blocks up to and with each tile
   int reqs[kMaxSplitTiles];
-  int sums[kWaves];
-  int flag[2];
+  int sums[8];
+  int flag[2];                         // some row's maximum passed its reference
   int first;
 };
 
@@ -115,11 +131,20 @@ __device__ __forceinline__ void load_lds16_at(uint32_t dst, const uint8_t* p) {
 // of a transposing read (two neighbouring chunks each) four different pairs.
 __device__ __forceinline__ int swizzle(int key) { return ((key & 3) << 1) | ((key >> 2) & 1); }
 
+// Maximum and sum over a row's lanes: four of 16 apart (quad), two of 32 (half).
 __device__ __forceinline__ float quad_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_max(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 __device__ __forceinline__ float quad_sum(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -128,15 +153,15 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Eight INT8 codes as eight bf16 (exact).
+// Eight INT8 codes as eight bf16 (exact): code + 128 by the byte conversions,
+// which run at the full rate (the signed conversion does at a quarter of it).
 __device__ __forceinline__ uint4 codes_to_bf16(uint2 v) {
   uint32_t o[4];
-  const uint32_t w[2] = {v.x, v.y};
+  const uint32_t w[2] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u};
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const int32_t x = static_cast<int32_t>(w[k]);
-    const float f0 = static_cast<float>((x << 24) >> 24), f1 = static_cast<float>((x << 16) >> 24);
-    const float f2 = static_cast<float>((x << 8) >> 24), f3 = static_cast<float>(x >> 24);
+    const float f0 = static_cast<float>(w[k] & 0xffu) - 128.f, f1 = static_cast<float>(w[k] >> 8 & 0xffu) - 128.f;
+    const float f2 = static_cast<float>(w[k] >> 16 & 0xffu) - 128.f, f3 = static_cast<float>(w[k] >> 24) - 128.f;
     o[2 * k] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
     o[2 * k + 1] = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u);
   }
@@ -150,36 +175,23 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
   return w;
 }
 
-// One K-step's products of four row tiles, the queries in accumulation
-// registers (kAcc) or vector ones; with kFirst the sums start at 0.  In asm
-// because the compiler, with nearly all 512 registers of a lane in use, copies
-// the queries to vector registers before most products otherwise.  The two
-// wait states before the products are what a vector instruction that wrote
-// one of their operands needs; nothing but these products writes s, and
-// products_done() comes before its first other use.
-template <bool kFirst, bool kAcc>
-__device__ __forceinline__ void four_products(f32x4 (&s)[4], bf16x8 k, bf16x8 q0, bf16x8 q1, bf16x8 q2, bf16x8 q3) {
+// One K-step's product of 32 keys and 32 rows, the queries in accumulation
+// registers; with kFirst the sum starts at 0.  In asm because the compiler,
+// with most of a lane's 512 registers in use, otherwise copies the queries to
+// vector registers before the products.  The two wait states before the
+// product are what a vector instruction that wrote one of its operands needs;
+// nothing but these products writes s, and product_done() comes before its
+// first other use.
+template <bool kFirst>
+__device__ __forceinline__ void product(f32x16& s, bf16x8 k, bf16x8 q) {
   if constexpr (kFirst)
-    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, 0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, 0\n\t"
-        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, 0\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, 0"
-        : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-        : "v"(k), "a"(q0), "a"(q1), "a"(q2), "a"(q3));
-  else if constexpr (kAcc)
-    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, %1\n\t"
-        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, %3"
-        : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])
-        : "v"(k), "a"(q0), "a"(q1), "a"(q2), "a"(q3));
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "a"(q));
   else
-    asm("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %4, %5, %0\n\tv_mfma_f32_16x16x32_bf16 %1, %4, %6, %1\n\t"
-        "v_mfma_f32_16x16x32_bf16 %2, %4, %7, %2\n\tv_mfma_f32_16x16x32_bf16 %3, %4, %8, %3"
-        : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3])
-        : "v"(k), "v"(q0), "v"(q1), "v"(q2), "v"(q3));
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "a"(q));
 }
-// Wait states between a product and a vector instruction that reads it (11
-// for products of this shape; 16 here).
-__device__ __forceinline__ void products_done(f32x4 (&s)[4]) {
-  asm volatile("s_nop 15" : "+v"(s[0]), "+v"(s[1]), "+v"(s[2]), "+v"(s[3]));
-}
+// Wait states between a product and a vector instruction that reads it (19
+// for the longest products; 24 here).
+__device__ __forceinline__ void product_done(f32x16& s) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s)); }
 
 // What a request's tokens and keys are, from values that may be anything:
 // token ranges are clipped to the queries there are, lengths to the table.
@@ -213,25 +225,37 @@ __device__ __forceinline__ int last_key(const Request& r, int row0, int heads, i
 
 // The kernel's arguments read where they are used, instead of being kept in
 // scalar registers from the start.
-__device__ __forceinline__ const ChunkArgs& late_args() {
+typedef const __attribute__((address_space(4))) ChunkArgs LateArgs;
+__device__ __forceinline__ LateArgs* late_args() {
   uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return *(const ChunkArgs*)p;
+  return (LateArgs*)p;
 }
 
 template <int kTM, bool kInt8, bool kSplit>
-__global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
-  constexpr int kRT = kTM / 16;              // row tiles
-  constexpr int kSteps = kInt8 ? 16 : 18;    // K-steps of 32
+__global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
+  using Shape = ChunkShape<kTM>;
+  constexpr bool kBig = Shape::kBig;
+  constexpr int kWaves = Shape::kWaves, kThreads = Shape::kThreads, kOwn = Shape::kOwn;
+  constexpr int kRowSize = kBig ? 32 : 16;         // rows and latents of a product
+  constexpr int kRT = kTM / kRowSize;              // row tiles
+  constexpr int kLT = kLatent / kRowSize / kWaves; // PV: latent tiles of a wave
+  constexpr int kDepth = kBig ? 16 : 32;           // K-step of a product
+  constexpr int kSteps = (kInt8 ? kLatent : kLatent + kRope) / kDepth;
+  constexpr int kPvSteps = kLT * kKeys / kDepth;
+  constexpr int kLoads = kOwn + (kInt8 ? 0 : kOwn / 8);   // loads a wave sends per block
+  using Acc = std::conditional_t<kBig, f32x16, f32x4>;
+  constexpr int kAcc = kBig ? 16 : 4;
   __shared__ ChunkShared<kTM> sh;
 
   const int w = uniform(threadIdx.x >> 6);
   int lane = threadIdx.x & 63;
   // What depends on the lane alone would be kept in registers across the
-  // block loop, which has none to spare: forget() makes the compiler derive it
-  // anew from the lane.
+  // block loop; forget() makes the compiler derive it anew from the lane.
   auto forget = [&]() { asm volatile("" : "+v"(lane)); };
-  int g = lane >> 4, c = lane & 15;
+  // QK: the wave's key group (32 or 16 keys) and row tile
+  const int kg = kBig ? w & 1 : w & 3, rh = kBig ? w >> 1 : w >> 2;
+  const bool takes_rows = rh < kRT;
   const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.block_size;
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
@@ -249,7 +273,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     for (int k = 0; k < kTiles; k++) {
       const int t = static_cast<int>(threadIdx.x) * kTiles + k;
       int at = 0;                                       // the last request that starts at or before tile t
-      for (int step = kMaxSplitTiles / 2; step; step >>= 1) {
+      for (int step = a.first_step; step; step >>= 1) {
         const int r = at + step;
         if (r < a.num_reqs && first_tile<kTM>(cu_s[r], a.heads, r) <= t) at = r;
       }
@@ -305,8 +329,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 
   for (;; tile++) {
     // ---- the tile: its request, its rows, its blocks [b0, b1)
-    int r, b0, b1, start = 0, units;
-    Request rq;
+    int r, b0 = 0, b1 = 0, start = 0, units = 0;
     if (kSplit) {
       if (tile >= kMaxSplitTiles) return;
       start = tile ? uniform(sh.ends[tile - 1]) : 0;
@@ -319,43 +342,42 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       b1 = min(hi - start, units);
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
-      int count = 0;
+      int begun = 0;
       for (int i = threadIdx.x; i < a.num_reqs; i += kThreads)
-        count += first_tile<kTM>(min(max(a.cu[i], 0), a.total_q), a.heads, i) <= tile;
+        begun += first_tile<kTM>(min(max(a.cu[i], 0), a.total_q), a.heads, i) <= tile;
 #pragma unroll
-      for (int d = 32; d; d >>= 1) count += __shfl_xor(count, d);
-      if (lane == 0) sh.sums[w] = count;
+      for (int d = 32; d; d >>= 1) begun += __shfl_xor(begun, d);
+      if (lane == 0) sh.sums[w] = begun;
       wg_barrier();
       r = -1;
 #pragma unroll
       for (int i = 0; i < kWaves; i++) r += sh.sums[i];
       r = uniform(max(r, 0));
-      b0 = b1 = units = 0;
     }
-    rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
+    const Request rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
     const int last = last_key<kTM>(rq, row0, a.heads, max_pos);
-    if (!kSplit) {
-      units = b1 = last >= 0 ? last / kKeys + 1 : 0;
-    } else if (last < 0) {
+    if (!kSplit)
+      b1 = last >= 0 ? last / kKeys + 1 : 0;
+    else if (last < 0)
       b1 = b0;   // nothing to see: its one unit writes the zeros
-    }
     // the least of the rows' last positions: keys past it are masked for some row
     const int64_t least64 = static_cast<int64_t>(rq.len) - rq.n + row0 / a.heads;
     const int least = static_cast<int>(least64 < -1 ? -1 : least64 < last ? least64 : last);
 
-    if (kSplit) wg_barrier();   // the buffers are free (the tile before, the scan)
+    if (kSplit) wg_barrier();   // LDS is free (the tile before, the scan)
 
-    // ---- bringing blocks in.  Wave w brings in the 16 keys that it takes in
-    // QK.  Lane c (of each 16) looks up key 16 w + c: its page in the table,
-    // one block ahead of its use, then its row's address.  A key past the
-    // sequence, or whose page is not in the table or the cache, has none: the
-    // cache's first row is read in its place and zeroed.
+    // ---- bringing blocks in.  Wave w brings in the rows of keys kOwn w ... .
+    // Lane c (of each kOwn) looks up key kOwn w + c: its page in the table, one
+    // block ahead of its use, then its row's address.  A key past the last one
+    // seen, or whose page is not in the table or the cache, has no row: the
+    // cache's first is read in its place and zeroed.  After the last block
+    // there are no rows, and the loads bring nothing that is used.
     uint2 codes[kInt8 ? kOwn : 1];
     float scale = 0.f;
-    int pos = b0 * kKeys + kOwn * w + c;   // of the block that `page` is for
+    int pos = b0 * kKeys + kOwn * w + (lane & (kOwn - 1));   // of the block that `page` is for
     int pg = pos / a.block_size, in_page = pos - pg * a.block_size, page = -1;
     const int step_pg = kKeys / a.block_size, step_in = kKeys - step_pg * a.block_size;
     const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
@@ -366,18 +388,22 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       in_page += step_in;
       if (in_page >= a.block_size) in_page -= a.block_size, pg++;
     };
-    uint32_t row_lo = 0, row_hi = 0, have = 0, have_next = 0;   // addresses; bit j: key 16 w + j has a row
-    auto address = [&]() {
+    uint32_t row_lo = 0, row_hi = 0, mine = 0;   // addresses; bit j: this wave's row j is there
+    constexpr uint32_t kAll = (1u << kOwn) - 1;
+    auto address = [&](int b) {
       const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
-      have_next = static_cast<uint32_t>(__ballot(ok)) & 0xffff;
+      mine = static_cast<uint32_t>(__ballot(ok)) & kAll;
       const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
                           (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
       row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
+      if (lane == 0) {
+        if constexpr (kBig)
+          reinterpret_cast<uint16_t*>(&sh.have[b & 1])[w] = static_cast<uint16_t>(mine);
+        else
+          reinterpret_cast<uint8_t*>(&sh.have[b & 1])[w] = static_cast<uint8_t>(mine);
+      }
     };
-    // Step j of kSteps of bringing in block b.  With 64 rows the products
-    // bound the loop, and the loads are spread over it: sent at once they
-    // fill the CU's miss queue and hold up the products behind them.
-    constexpr bool kSpread = kRT == 4 && !kInt8;
+    // load j of kLoads of block b
     auto bring = [&](int b, int j) {
       auto& blk = sh.kv[b & 1];
       if (j < kOwn) {
@@ -398,70 +424,70 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       if (kInt8 && j == kOwn - 1)
         scale = *reinterpret_cast<const float*>((row_lo | static_cast<uint64_t>(row_hi) << 32) + kLatent);
     };
-    // INT8: row j of the wave's keys of block b as bf16 into LDS (0 without a row)
+    // INT8: row j of the wave's rows of block b as bf16 into LDS (0 without a row)
     auto put_row = [&](int b, int j) {
       if constexpr (kInt8) {
-        const uint2 v = have_next >> j & 1 ? codes[j] : make_uint2(0, 0);
-        *reinterpret_cast<uint4*>(&sh.kv[b & 1].lat[kOwn * w + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
-        if (j == kOwn - 1 && lane < kOwn) sh.scl[b & 1][kOwn * w + lane] = have_next >> lane & 1 ? scale : 0.f;
+        const uint32_t keep = 0u - (mine >> j & 1);
+        *reinterpret_cast<uint4*>(&sh.kv[b & 1].lat[kOwn * w + j][(16 * lane) ^ (16 * swizzle(j))]) =
+            codes_to_bf16(make_uint2(codes[j].x & keep, codes[j].y & keep));
+        if (j == kOwn - 1 && lane < kOwn) sh.scl[b & 1][kOwn * w + lane] = mine >> lane & 1 ? scale : 0.f;
       }
     };
 
     if (b0 < b1) {
       look_up(b0);
-      address();
+      address(b0);
       advance();
 #pragma unroll
-      for (int j = 0; j < kSteps; j++) bring(b0, j);
+      for (int j = 0; j < kLoads; j++) bring(b0, j);
       look_up(b0 + 1);
     }
 
-    // ---- the queries: row c of row tile rt (rows past the last: the last,
-    // not stored).  Every wave needs all of them, so they come through LDS
-    // once, in the buffer that the second block will take, laid out like keys:
-    // wave w brings in every fourth row.
-    bf16x8 qf[kRT][kSteps];
+    // ---- the queries (rows past the last: the last, not stored).  Several
+    // waves need each, so they come through LDS once, in the buffer that the
+    // second block will take, laid out like keys: wave w brings in every
+    // kWaves-th row.
+    bf16x8 qf[kSteps];
     {
       auto& qs = sh.kv[(b0 + 1) & 1];
       constexpr int kMine = kTM / kWaves;
-      const int row = min(row0 + kWaves * min(c, kMine - 1) + w, rows - 1);
+      const int row = min(row0 + kWaves * min(lane & 15, kMine - 1) + w, rows - 1);
       const int tok = row / a.heads, head = row - tok * a.heads;
       const uint64_t at = reinterpret_cast<uint64_t>(a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t +
                                                      static_cast<int64_t>(head) * a.sq_h);
       const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
 #pragma unroll
       for (int j = 0; j < kMine; j++) {
-        const uint64_t from = static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, j)) |
-                              static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, j))) << 32;
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, j)) |
+            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, j))) << 32);
         const int key = kWaves * j + w;
-        load_lds16(lds_offset(qs.lat[key]), reinterpret_cast<const uint8_t*>(from), 16 * (lane ^ swizzle(key)));
+        load_lds16(lds_offset(qs.lat[key]), from, 16 * (lane ^ swizzle(key)));
         if constexpr (!kInt8) {
-          if (lane < 8)
-            load_lds16(lds_offset(qs.rope[key]), reinterpret_cast<const uint8_t*>(from),
-                       2 * kLatent + 16 * (lane ^ swizzle(key)));
+          if (lane < 8) load_lds16(lds_offset(qs.rope[key]), from, 2 * kLatent + 16 * (lane ^ swizzle(key)));
         }
       }
       loads_done();   // the queries, and the first block's rows
       wg_barrier();
+      const int key = kRowSize * (takes_rows ? rh : 0) + (lane & (kRowSize - 1)), sw = swizzle(lane), part = lane / kRowSize;
+      constexpr int kChunks = kDepth / 8;   // 16-byte chunks of a K-step
 #pragma unroll
-      for (int rt = 0; rt < kRT; rt++) {
-        const int key = 16 * rt + c, sw = swizzle(c);
-#pragma unroll
-        for (int st = 0; st < kSteps; st++) {
-          const uint8_t* from = st < 16 ? qs.lat[key] + 16 * ((4 * (st & 1) + g) ^ sw) + 128 * (st >> 1)
-                                        : qs.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
-          qf[rt][st] = *reinterpret_cast<const bf16x8*>(from);
-        }
+      for (int st = 0; st < kSteps; st++) {
+        const int chunk = kChunks * st;     // + part
+        const uint8_t* from = chunk < 64 ? qs.lat[key] + 16 * (((chunk & 7) + part) ^ sw) + 128 * (chunk >> 3)
+                                         : qs.rope[key] + 16 * ((chunk - 64 + part) ^ sw);
+        qf[st] = *reinterpret_cast<const bf16x8*>(from);
       }
     }
-    f32x4 acc[kLT][kRT];
+    Acc acc[kLT][kRT];
 #pragma unroll
     for (int i = 0; i < kLT; i++)
 #pragma unroll
-      for (int j = 0; j < kRT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref[kRT], sum[kRT];
+      for (int j = 0; j < kRT; j++)
 #pragma unroll
-    for (int rt = 0; rt < kRT; rt++) ref[rt] = -INFINITY, sum[rt] = 0.f;
+        for (int e = 0; e < kAcc; e++) acc[i][j][e] = 0.f;
+    // the reference maximum (log2) of this lane's row, from the least number on: every other logit passes it
+    float ref = -3.4028234663852886e38f, sum = 0.f;
     if (b0 < b1) {
 #pragma unroll
       for (int j = 0; j < kOwn; j++) put_row(b0, j);
@@ -470,147 +496,174 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 
     for (int b = b0; b < b1; b++) {
       loads_done();   // this wave's rows of block b
-      wg_barrier();   // nobody reads the other buffer, P or the maxima any more
-      have = have_next;
       auto& blk = sh.kv[b & 1];
-      forget();
-      g = lane >> 4, c = lane & 15;
-      if (!kInt8 && have != 0xffff) {
+      if (!kInt8 && mine != kAll) {
         for (int j = 0; j < kOwn; j++)
-          if (!(have >> j & 1)) {
+          if (!(mine >> j & 1)) {
             *reinterpret_cast<uint4*>(&blk.lat[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
             if (lane < 8) *reinterpret_cast<uint4*>(&blk.rope[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
           }
       }
+      wg_barrier();   // every wave's rows are there; nobody reads the other buffer, P or the maxima any more
+      forget();
       if (w == 0 && lane == 0) sh.flag[(b + 1) & 1] = 0;
+      const uint64_t have_v = sh.have[b & 1];
+      address(b + 1);
 
-      // ---- S^T = K Q^T: keys 16 w + 4 g + i of the block, rows c.  Each
-      // K-step's operand is read kAhead steps before its products, and between
-      // the steps a row of the next block is asked for.
-      f32x4 s[kRT];
-      if constexpr (kRT != 4) {
+      // ---- S^T = K Q^T: the wave's keys, one row a lane.  Each K-step's
+      // operand is read some steps before its product; between the steps the
+      // next block's rows are asked for - all of them here where memory bounds
+      // the loop, and spread over the block where the products do: sent at
+      // once they fill the CU's miss queue and hold up the products behind.
+      constexpr int kInQk = kBig && !kInt8 ? 12 : kLoads, kInSm = kBig && !kInt8 ? 3 : 0;
+      Acc s;
+      if (takes_rows) {
+        constexpr int kRead = kBig ? 6 : 5, kChunks = kDepth / 8;
+        const int key = kRowSize * kg + (lane & (kRowSize - 1)), sw = swizzle(lane), part = lane / kRowSize;
+        const uint8_t* base[8 / kChunks];
 #pragma unroll
-        for (int rt = 0; rt < kRT; rt++) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      address();   // after the last block: no rows, the cache's first in their place
-      {
-        constexpr int kAhead = 5;
-        const int key = kOwn * w + c, sw = swizzle(c);
-        const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
-        const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
+        for (int i = 0; i < 8 / kChunks; i++) base[i] = blk.lat[key] + 16 * ((kChunks * i + part) ^ sw);
         const uint8_t* rope = blk.rope[key];
         auto operand = [&](int st) {
-          return *reinterpret_cast<const bf16x8*>(st < 16 ? (st & 1 ? odd : even) + 128 * (st >> 1)
-                                                          : rope + 16 * ((4 * (st - 16) + g) ^ sw));
+          const int chunk = kChunks * st;
+          return *reinterpret_cast<const bf16x8*>(chunk < 64 ? base[st % (8 / kChunks)] + 128 * (chunk >> 3)
+                                                             : rope + 16 * ((chunk - 64 + part) ^ sw));
         };
         bf16x8 k[kSteps];
+        Acc odd;
 #pragma unroll
-        for (int st = 0; st < kAhead; st++) k[st] = operand(st);
+        for (int e = 0; e < kAcc; e++) odd[e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < kRead; st++) k[st] = operand(st);
 #pragma unroll
         for (int st = 0; st < kSteps; st++) {
-          if (st + kAhead < kSteps) k[st + kAhead] = operand(st + kAhead);
-          if constexpr (kRT == 4) {
+          if (st + kRead < kSteps) k[st + kRead] = operand(st + kRead);
+          if constexpr (kBig) {
             if (st == 0)
-              four_products<true, true>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
-            else if (st < 16)
-              four_products<false, true>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
+              product<true>(s, k[st], qf[st]);
             else
-              four_products<false, false>(s, k[st], qf[0][st], qf[1][st], qf[2][st], qf[3][st]);
-          } else {
+              product<false>(s, k[st], qf[st]);
+            if (kInt8 ? st % 2 == 0 : st % 3 == 0) bring(b + 1, kInt8 ? st / 2 : st / 3);
+          } else {   // two sums, so that a product does not wait for the one before it
+            if (st == 0)
 #pragma unroll
-            for (int rt = 0; rt < kRT; rt++)
-              s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], s[rt], 0, 0, 0);
+              for (int e = 0; e < kAcc; e++) s[e] = 0.f;
+            if (st & 1)
+              odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[st], odd, 0, 0, 0);
+            else
+              s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[st], s, 0, 0, 0);
+            if (st < kLoads) bring(b + 1, st);
           }
-          if (!kSpread || st % 2 == 0) bring(b + 1, kSpread ? st / 2 : st);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (kRT == 4) products_done(s);
+        if constexpr (kBig) {
+          product_done(s);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kAcc; e++) s[e] += odd[e];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) bring(b + 1, j);
       }
-      if (kSpread) bring(b + 1, 9), bring(b + 1, 10);
-
       forget();
-      g = lane >> 4, c = lane & 15;
-      const bool masked = (b + 1) * kKeys - 1 > least || have != 0xffff;   // uniform
-      float ksv[4] = {1.f, 1.f, 1.f, 1.f};
-      if constexpr (kInt8) {
-        const float4 ks = *reinterpret_cast<const float4*>(&sh.scl[b & 1][kOwn * w + 4 * g]);
-        ksv[0] = ks.x, ksv[1] = ks.y, ksv[2] = ks.z, ksv[3] = ks.w;
-      }
+
+      // ---- softmax.  Element e of a lane is key key_of(e) of the block, its
+      // row c of row tile rh.
+      const int part = lane / kRowSize, c = lane & (kRowSize - 1);
+      auto key_of = [&](int e) { return kRowSize * kg + (kBig ? 8 * (e >> 2) + 4 * part + (e & 3) : 4 * part + e); };
+      float weights = 0.f;
+      float ksv[kInt8 ? kAcc : 1];
+      auto put_p = [&]() {
+        float p[kAcc];
 #pragma unroll
-      for (int rt = 0; rt < kRT; rt++)
+        for (int e = 0; e < kAcc; e++) p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
+        float t[kAcc / 4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[rt][i] *= kInt8 ? a.scale_log2 * ksv[i] : a.scale_log2;
-      if (masked) {
+        for (int e = 0; e < kAcc; e += 4) t[e / 4] = (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
+        weights = kBig ? (t[0] + t[1 % (kAcc / 4)]) + (t[2 % (kAcc / 4)] + t[3 % (kAcc / 4)]) : t[0];
+        if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
 #pragma unroll
-        for (int rt = 0; rt < kRT; rt++) {
-          const int row = min(row0 + 16 * rt + c, rows - 1);
+          for (int e = 0; e < kAcc; e++) p[e] *= ksv[e];
+        }
+        // P is rounded to bf16 (like the output, 2^-9 of each weight on the
+        // average); the sum keeps the unrounded weights.  Chunk of 8 keys and
+        // half: with the small products the operand's keys of each 32 are
+        // 4 g + i and 16 + 4 g + i.
+        uint8_t* row = sh.p[kRowSize * rh + c];
+#pragma unroll
+        for (int e = 0; e < kAcc; e += 4) {
+          const int chunk = kBig ? 4 * kg + e / 4 : 4 * (kg >> 1) + part, half = kBig ? part : kg & 1;
+          *reinterpret_cast<uint2*>(row + 16 * (chunk ^ (c & 7)) + 8 * half) =
+              make_uint2(pack_bf16x2(p[e], p[e + 1]), pack_bf16x2(p[e + 2], p[e + 3]));
+        }
+      };
+      if (takes_rows) {
+        const uint64_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v))) |
+                              static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(have_v >> 32)))) << 32;
+        if constexpr (kInt8) {
+#pragma unroll
+          for (int e = 0; e < kAcc; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&sh.scl[b & 1][key_of(e)]);
+            ksv[e] = v.x, ksv[e + 1] = v.y, ksv[e + 2] = v.z, ksv[e + 3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kAcc; e++) s[e] *= kInt8 ? a.scale_log2 * ksv[kInt8 ? e : 0] : a.scale_log2;
+        if (have != ~0ull || (b + 1) * kKeys - 1 > least) {
+          const int row = min(row0 + kRowSize * rh + c, rows - 1);
           const int64_t see = static_cast<int64_t>(rq.len) - rq.n + row / a.heads;
           const int limit = static_cast<int>(see < last ? see < -1 ? -1 : see : last) - b * kKeys;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int k = 4 * g + i;
-            if (kOwn * w + k > limit || !(have >> k & 1)) s[rt][i] = -INFINITY;
+          for (int e = 0; e < kAcc; e++) {
+            const int k = key_of(e);
+            if (k > limit || !(have >> k & 1)) s[e] = -INFINITY;
           }
         }
-      }
-      float top[kRT], mine = 0.f;
-      bool moved = false;
+        if constexpr (kInt8) {
+          // a scale that is not a number has made its logits so; where it is
+          // masked, the weight 0 has to stay 0
 #pragma unroll
-      for (int rt = 0; rt < kRT; rt++) {
-        top[rt] = quad_max(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3])));
-        moved |= top[rt] > ref[rt] + kSlack;
-        if (g == rt) mine = top[rt];
-      }
-      if (lane < kTM) sh.red[w][lane] = mine;   // row 16 g + c
-      if (__ballot(moved) && lane == 0) sh.flag[b & 1] = 1;
-
-      // P of this wave's keys, against the reference (0 where a row has seen nothing)
-      float part[kRT];
-      auto put_p = [&]() {
-#pragma unroll
-        for (int rt = 0; rt < kRT; rt++) {
-          const float m = ref[rt] == -INFINITY ? 0.f : ref[rt];
-          float p[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(s[rt][i] - m);
-          part[rt] = (p[0] + p[1]) + (p[2] + p[3]);
-          if constexpr (kInt8) {
-            // V = codes * scale: the scale goes to P, which a masked key has as 0 whatever its scale is
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = s[rt][i] == -INFINITY ? 0.f : p[i] * ksv[i];
-          }
-          // P is rounded to bf16 (2^-9 of each weight on the average, like the
-          // output's own rounding); the sum keeps the unrounded weights
-          *reinterpret_cast<uint2*>(&sh.p[16 * rt + c][64 * (w >> 1) + 16 * g + 8 * (w & 1)]) =
-              make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
+          for (int e = 0; e < kAcc; e++) ksv[e] = fabsf(ksv[e]) < INFINITY ? ksv[e] : 0.f;
         }
-      };
-      put_p();
-      if (kSpread) bring(b + 1, 11), bring(b + 1, 12);
+        if (kInSm > 0) bring(b + 1, kInQk);
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < kAcc; e++) top = fmaxf(top, s[e]);
+        top = kBig ? half_max(top) : quad_max(top);
+        if (lane < kRowSize) sh.red[kg][kRowSize * rh + c] = top;
+        if (__ballot(top > ref + kSlack) && lane == 0) sh.flag[b & 1] = 1;
+        if (kInSm > 1) bring(b + 1, kInQk + 1);
+        put_p();
+        if (kInSm > 2) bring(b + 1, kInQk + 2);
+      }
       advance();
       look_up(b + 2);
-      wg_barrier();   // P is whole; every wave's rows are there
+      wg_barrier();   // P is whole
 
       if (uniform(sh.flag[b & 1])) {   // some row's maximum passed its reference: all rows take theirs
+        if (takes_rows) {
+          const int row = kRowSize * rh + c;
+          float m = ref;
 #pragma unroll
-        for (int rt = 0; rt < kRT; rt++) {
-          const int row = 16 * rt + c;
-          float m = ref[rt];
+          for (int i = 0; i < kKeys / kRowSize; i++) m = fmaxf(m, sh.red[i][row]);
+          const float alpha = __builtin_amdgcn_exp2f(ref - m);
+          ref = m;
+          sum *= alpha;
+          if (kg == 0 && lane < kRowSize) sh.ref[row] = alpha;
+          put_p();
+        }
+        wg_barrier();
 #pragma unroll
-          for (int i = 0; i < kWaves; i++) m = fmaxf(m, sh.red[i][row]);
-          const float alpha = __builtin_amdgcn_exp2f(ref[rt] - (m == -INFINITY ? 0.f : m));
-          ref[rt] = m;
-          sum[rt] *= alpha;
+        for (int j = 0; j < kRT; j++) {
+          const float alpha = sh.ref[kRowSize * j + c];
 #pragma unroll
           for (int i = 0; i < kLT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[i][rt][e] *= alpha;
+            for (int e = 0; e < kAcc; e++) acc[i][j][e] *= alpha;
         }
-        put_p();
-        wg_barrier();
       }
-#pragma unroll
-      for (int rt = 0; rt < kRT; rt++) sum[rt] += part[rt];
+      sum += weights;
 
       if constexpr (!kInt8) {
         // Keys that some row of the tile may not see: 0 * inf would put NaN
@@ -624,133 +677,170 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           wg_barrier();
         }
       }
-
       forget();
-      g = lane >> 4, c = lane & 15;
-      // ---- O^T += V^T P^T: latents 16 (kLT w + i) + 4 g + e, rows 16 j + c;
-      // V's operands two steps ahead.  INT8: a row of the next block is
-      // converted between the steps.
+
+      // ---- O^T += V^T P^T: the wave's latent tiles, all rows; V's operands are
+      // read some steps ahead.  INT8: a row of the next block is converted
+      // between the steps.
       {
-        constexpr int kPv = 2 * kLT, kAhead = 3;
-        const int tr_row = 4 * g + (c >> 2), tr_sw = swizzle(tr_row);
-        const uint8_t* vr[4];
+        constexpr int kRead = kBig ? 4 : 3, kGroups = kKeys / kDepth;
+        const int g = lane >> 4, c16 = lane & 15;
+        // a transposing read gives a lane its column (latent) of four rows (keys)
+        const int tr_row = kBig ? 8 * (lane >> 5) + (c16 >> 2) : 4 * g + (c16 >> 2);
+        const int tr_col = (kBig ? 2 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
+        constexpr int kTileChunks = kRowSize / 8, kBases = 8 / kTileChunks;  // the swizzle is on 8 chunks
+        constexpr int kSecond = (kBig ? 4 : 16) * 2 * kLatent;               // rows of the operand's other half
+        const uint8_t* base[kBases][kBig ? 2 : 1];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          vr[i] = &blk.lat[tr_row][256 * w + 16 * ((2 * i + ((c & 3) >> 1)) ^ tr_sw) + 8 * (c & 1)];
+        for (int i = 0; i < kBases; i++)
+#pragma unroll
+          for (int h = 0; h < (kBig ? 2 : 1); h++)
+            base[i][h] = &blk.lat[tr_row + 4 * h][128 * (kLT * kTileChunks * w / 8) +
+                                                  16 * ((kTileChunks * i + tr_col) ^ swizzle(tr_row + 4 * h)) + 8 * (c16 & 1)];
         auto operand = [&](int u) {
-          const uint8_t* p = vr[u & 3] + 128 * (u >> 2 & 1) + 32 * 2 * kLatent * (u >> 3);
-          const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p)));
-          const i32x2 v1 = __builtin_bit_cast(
-              i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p + 16 * 2 * kLatent)));
+          const int i = u % kLT, t = u / kLT;   // latent tile, keys
+          const int off = 128 * (i / kBases) + kDepth * t * 2 * kLatent;
+          const uint8_t* p0 = base[i % kBases][0] + off;
+          const uint8_t* p1 = kBig ? base[i % kBases][kBig ? 1 : 0] + off : p0 + kSecond;
+          const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p0)));
+          const i32x2 v1 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p1)));
           return __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
         };
-        bf16x8 pb[2][kRT], v[kPv];
+        auto weights_of = [&](int t, int j) {
+          const int chunk = kDepth / 8 * t + part;
+          return *reinterpret_cast<const bf16x8*>(sh.p[kRowSize * j + c] + 16 * (chunk ^ (c & 7)));
+        };
+        bf16x8 pb[kGroups][kRT], v[kPvSteps];
 #pragma unroll
-        for (int j = 0; j < kRT; j++) pb[0][j] = *reinterpret_cast<const bf16x8*>(&sh.p[16 * j + c][16 * g]);
+        for (int j = 0; j < kRT; j++) pb[0][j] = weights_of(0, j);
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) v[u] = operand(u);
+        for (int u = 0; u < kRead; u++) v[u] = operand(u);
 #pragma unroll
-        for (int u = 0; u < kPv; u++) {
-          if (u + kAhead < kPv) v[u + kAhead] = operand(u + kAhead);
-          if (u >= kLT - kRT && u < kLT) {
-            const int j = u - (kLT - kRT);
-            pb[1][j] = *reinterpret_cast<const bf16x8*>(&sh.p[16 * j + c][64 + 16 * g]);
+        for (int u = 0; u < kPvSteps; u++) {
+          const int i = u % kLT, t = u / kLT;
+          if (u + kRead < kPvSteps) v[u + kRead] = operand(u + kRead);
+          if (i < kRT && t + 1 < kGroups) pb[t + 1][i] = weights_of(t + 1, i);
+#pragma unroll
+          for (int j = 0; j < kRT; j++) {
+            if constexpr (kBig)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
+            else
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
           }
-#pragma unroll
-          for (int j = 0; j < kRT; j++)
-            acc[u % kLT][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[u / kLT][j], acc[u % kLT][j], 0, 0, 0);
-          if (kSpread && u < 5) bring(b + 1, 13 + u);
-          put_row(b + 1, u);
+          if (u < kLoads - kInQk - kInSm) bring(b + 1, kInQk + kInSm + u);
+          if (kInt8 && u < kOwn) put_row(b + 1, u);
           __builtin_amdgcn_sched_barrier(0);
         }
+        static_assert(kOwn <= kPvSteps && kLoads - kInQk - kInSm <= kPvSteps, "every row has its step");
       }
     }
-    loads_done();   // what the last block asked for
+    loads_done();   // what was asked for past the last block
 
     // ---- the rows' sums and references, then the output or the partial
     wg_barrier();
-#pragma unroll
-    for (int rt = 0; rt < kRT; rt++) {
-      const float l = quad_sum(sum[rt]);
-      if (g == 0) sh.red[w][16 * rt + c] = l;
-      if (w == 0 && g == 0) sh.ref[16 * rt + c] = ref[rt];
+    const int part = lane / kRowSize, c = lane & (kRowSize - 1);
+    if (takes_rows) {
+      const float l = kBig ? half_sum(sum) : quad_sum(sum);
+      const int row = kRowSize * rh + c;
+      if (lane < kRowSize) sh.red[kg][row] = l;
+      if (kg == 0 && lane < kRowSize) sh.ref[row] = ref;
     }
     wg_barrier();
-    const ChunkArgs& e = late_args();
+    auto sum_of = [&](int row) {
+      float l = sh.red[0][row] + sh.red[1][row];
+      if (!kBig) l += sh.red[2][row] + sh.red[3][row];
+      return l;
+    };
+    LateArgs* e = late_args();
     if (!kSplit || (lo <= start && start + units <= hi)) {
-      // whole rows go out: the row tiles as bf16 through LDS (8 bytes of row
-      // c at 16-byte chunk ^ (c % 8), so that rows fall on different banks),
-      // then each wave stores every fourth row
-      uint8_t(*os)[2 * kLatent] = sh.kv[0].lat;
+      // whole rows go out: as bf16 through LDS (chunk c of row r at c ^ (r %
+      // 8), so that rows fall on different banks), then each wave stores every
+      // kWaves-th row
+      uint8_t* os = sh.kv[0].lat[0];
 #pragma unroll
       for (int j = 0; j < kRT; j++) {
-        const float l = (sh.red[0][16 * j + c] + sh.red[1][16 * j + c]) + (sh.red[2][16 * j + c] + sh.red[3][16 * j + c]);
+        const float l = sum_of(kRowSize * j + c);
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int i = 0; i < kLT; i++) {
-          const f32x4 v = acc[i][j];
-          *reinterpret_cast<uint2*>(&os[16 * j + c][((32 * (kLT * w + i) + 16 * (g >> 1)) ^ (16 * (c & 7))) + 8 * (g & 1)]) =
-              make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
-        }
+        for (int i = 0; i < kLT; i++)
+#pragma unroll
+          for (int q = 0; q < kAcc; q += 4) {
+            const Acc v = acc[i][j];
+            const int lat = kRowSize * (kLT * w + i) + (kBig ? 8 * (q / 4) : 0) + 4 * part;   // of v[q]
+            *reinterpret_cast<uint2*>(os + (kRowSize * j + c) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (c & 7))) + (2 * lat & 15)) =
+                make_uint2(pack_bf16x2(v[q] * inv, v[q + 1] * inv), pack_bf16x2(v[q + 2] * inv, v[q + 3] * inv));
+          }
       }
       wg_barrier();
+      const int heads = e->heads, aligned = e->out_align16;
+      const int64_t so_t = e->so_t, so_h = e->so_h;
+      uint16_t* out = e->out;
+      float* lse = e->lse;
       for (int j = w; j < kTM && row0 + j < rows; j += kWaves) {
-        const int row = row0 + j, tok = row / e.heads, head = row - tok * e.heads;
-        uint16_t* o = e.out + static_cast<int64_t>(rq.t0 + tok) * e.so_t + static_cast<int64_t>(head) * e.so_h;
-        const uint4 v = *reinterpret_cast<const uint4*>(&os[j][(16 * lane) ^ (16 * (j & 7))]);
-        if (e.out_align16) {
+        const int row = row0 + j, tok = row / heads, head = row - tok * heads;
+        uint16_t* o = out + static_cast<int64_t>(rq.t0 + tok) * so_t + static_cast<int64_t>(head) * so_h;
+        const uint4 v = *reinterpret_cast<const uint4*>(os + j * 2 * kLatent + ((16 * lane) ^ (16 * (j & 7))));
+        if (aligned) {
           reinterpret_cast<uint4*>(o)[lane] = v;
         } else {
           reinterpret_cast<uint2*>(o)[2 * lane] = make_uint2(v.x, v.y);
           reinterpret_cast<uint2*>(o)[2 * lane + 1] = make_uint2(v.z, v.w);
         }
-        if (e.lse && lane == 0) {
-          const float l = (sh.red[0][j] + sh.red[1][j]) + (sh.red[2][j] + sh.red[3][j]);
-          e.lse[static_cast<int64_t>(rq.t0 + tok) * e.heads + head] =
+        if (lse && lane == 0) {
+          const float l = sum_of(j);
+          lse[static_cast<int64_t>(rq.t0 + tok) * heads + head] =
               l == 0.f ? -INFINITY : (sh.ref[j] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
-      if (kSplit && threadIdx.x == 0) e.shares[tile] = make_int2(-1, -1);
+      if (kSplit && threadIdx.x == 0) e->shares[tile] = make_int2(-1, -1);
     } else {
-      // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins here
+      // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins
+      // here.  In the accumulators' order: 16 bytes of each lane at a time.
       const int slot = 2 * static_cast<int>(blockIdx.x) + (lo <= start);
-      float* part = e.part + static_cast<int64_t>(slot) * (kTM * kLatent);
+      float* out = e->part + static_cast<int64_t>(slot) * (kTM * kLatent);
 #pragma unroll
       for (int i = 0; i < kLT; i++)
 #pragma unroll
         for (int j = 0; j < kRT; j++)
-          *reinterpret_cast<f32x4*>(part + ((kLT * w + i) * kRT + j) * 256 + 4 * lane) = acc[i][j];
+#pragma unroll
+          for (int q = 0; q < kAcc; q += 4) {
+            const Acc v = acc[i][j];
+            *reinterpret_cast<f32x4*>(out + (((kLT * w + i) * kRT + j) * (kAcc / 4) + q / 4) * 256 + 4 * lane) =
+                f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+          }
       if (threadIdx.x < kTM) {
         const int row = threadIdx.x;
-        e.ml[static_cast<int64_t>(slot) * kTM + row] =
-            make_float2(sh.ref[row], (sh.red[0][row] + sh.red[1][row]) + (sh.red[2][row] + sh.red[3][row]));
+        e->ml[static_cast<int64_t>(slot) * kTM + row] = make_float2(sh.ref[row], sum_of(row));
       }
       if (lo <= start && threadIdx.x == 0) {
         const int64_t groups = min(static_cast<int>(gridDim.x), total);
         // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
         const int64_t last_unit = start + units;
-        e.shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
+        e->shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
       }
     }
     if (!kSplit) return;
   }
 }
 
-// Joins a shared tile's partials, 16 rows x 16 latents a job.  kTogether
+// Joins a shared tile's partials, 1 KB a job: 32 rows x 8 latents of a 64-row
+// tile, 16 x 16 of the others.  kTogether
 // waves take every kTogether-th partial each and join theirs through LDS (few
 // tiles, whose partials are many), or each of a workgroup's four waves takes a
 // job of its own.  kDeep partials are asked for at once.
 template <int kTM, int kTogether>
 __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(const ChunkArgs a) {
-  constexpr int kRT = kTM / 16, kDeep = 8;
+  constexpr int kRowSize = ChunkShape<kTM>::kBig ? 32 : 16, kRT = kTM / kRowSize, kQuads = kRowSize == 32 ? 4 : 1;
+  constexpr int kDeep = 8;
   __shared__ float acc_s[kTogether][64][4];
-  __shared__ float2 ml_s[kTogether][16];
+  __shared__ float2 ml_s[kTogether][kRowSize];
   const int tile = blockIdx.y;
   const int2 share = a.shares[tile];
   if (share.x < 0) return;
-  const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane / kRowSize, c = lane & (kRowSize - 1);
   const int job = kTogether > 1 ? blockIdx.x : 4 * blockIdx.x + w;
-  const int j = job % kRT, lt = job / kRT;
+  const int j = job / kQuads % kRT;   // row tile
+  const int lat = kRowSize * (job / (kQuads * kRT)) + 8 * (job % kQuads) + 4 * part;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   for (int k0 = share.x + (kTogether > 1 ? w : 0); k0 <= share.y; k0 += kTogether * kDeep) {
@@ -760,8 +850,8 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
     for (int d = 0; d < kDeep; d++) {
       const int k = min(k0 + kTogether * d, share.y);
       const int64_t slot = 2 * static_cast<int64_t>(k) + (k == share.x);
-      ml[d] = a.ml[slot * kTM + 16 * j + c];
-      v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + (lt * kRT + j) * 256 + 4 * lane);
+      ml[d] = a.ml[slot * kTM + kRowSize * j + c];
+      v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + job * 256 + 4 * lane);
     }
     float top = m;
 #pragma unroll
@@ -785,7 +875,7 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
   }
   if constexpr (kTogether > 1) {
     *reinterpret_cast<f32x4*>(acc_s[w][lane]) = acc;
-    if (g == 0) ml_s[w][c] = make_float2(m, l);
+    if (lane < kRowSize) ml_s[w][c] = make_float2(m, l);
     __syncthreads();
     if (w) return;
     float top = -INFINITY;
@@ -807,19 +897,19 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
   }
   // the request of the tile
   int at = 0;
-  for (int step = kMaxSplitTiles / 2; step; step >>= 1) {
+  for (int step = a.first_step; step; step >>= 1) {
     const int r = at + step;
     if (r < a.num_reqs && first_tile<kTM>(min(max(a.cu[r], 0), a.total_q), a.heads, r) <= tile) at = r;
   }
   const Request rq = request_of(a.cu[at], a.cu[at + 1], 0, a.total_q);
-  const int row = (tile - first_tile<kTM>(rq.t0, a.heads, at)) * kTM + 16 * j + c;
+  const int row = (tile - first_tile<kTM>(rq.t0, a.heads, at)) * kTM + kRowSize * j + c;
   if (row >= rq.n * a.heads) return;
   const int tok = row / a.heads, head = row - tok * a.heads;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* o = a.out + static_cast<int64_t>(rq.t0 + tok) * a.so_t + static_cast<int64_t>(head) * a.so_h;
-  *reinterpret_cast<uint2*>(o + 16 * lt + 4 * g) =
+  *reinterpret_cast<uint2*>(o + lat) =
       make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-  if (a.lse && lt == 0 && g == 0)
+  if (a.lse && lat == 0)
     a.lse[static_cast<int64_t>(rq.t0 + tok) * a.heads + head] =
         l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
@@ -851,14 +941,14 @@ Workspace workspace_of(int tm, int64_t tiles) {
 template <int kTM, bool kInt8>
 int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
   if (a.num_tiles > kMaxSplitTiles) {
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
     // a shared tile has about CUs / tiles partials: 16 waves on a job where
     // that is many, one where it is few
     if (a.num_tiles <= 16)
@@ -920,6 +1010,8 @@ extern "C" int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h, const 
   a.bt_stride = bt_stride;
   a.max_blocks = num_blocks > 0 ? static_cast<int>(max_blocks) : 0;
   a.block_size = static_cast<int>(block_size);
+  while (a.first_step < num_reqs && (a.first_step ? 2 * a.first_step : 1) < num_reqs)
+    a.first_step = a.first_step ? 2 * a.first_step : 1;
   a.num_reqs = static_cast<int>(num_reqs), a.total_q = static_cast<int>(total_q), a.heads = static_cast<int>(num_heads);
   a.num_tiles = static_cast<int>(tiles);
   a.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
