@@ -5,6 +5,7 @@ import fails loudly: there is no fallback implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -149,3 +150,21 @@ def check(rc: int, what: str) -> None:
 def stream_handle(device) -> int:
     import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device):
+    """torch.cuda.device(device), or nothing to enter where it is the current
+    device already (the context costs a small call 2 us)."""
+    import torch
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device) -> int:
+    """stream_handle without the Stream object around it, where torch offers
+    that (1 us of a small call)."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device.index) if get is not None else stream_handle(device)

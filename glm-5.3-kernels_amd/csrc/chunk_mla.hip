@@ -11,30 +11,30 @@
 //
 // Work: the (token, head) rows of a request are flattened and cut into tiles
 // of kTM rows (16, 32 or 64), which share every key they read; a tile walks
-// its keys in blocks of 64.  Per block, of one workgroup:
-//   * the block's rows come into LDS (bf16 rows by direct global -> LDS loads,
-//     INT8 rows converted to bf16 once), two buffers, the next block's loads
-//     on their way while this one is used;
-//   * S^T = K Q^T, the queries held in registers for the whole tile;
-//   * softmax against a reference maximum that moves only when some row's
-//     maximum passes it by 2^8 (sums and output are scaled to it in fp32), so
-//     that most blocks need no exchange of maxima between the two products;
-//   * O^T += V^T P^T, each wave its slice of the 512 latents for all rows: P
-//     goes through LDS as bf16, V is read from the same rows with transposing
-//     reads.
-// 64 rows are bound by the products.  Four waves, one per SIMD, so that a lane
-// has 512 registers (queries 144, output 128); products of 32 x 32 x 16, which
-// need half the instructions and operand reads of the small ones - a single
-// wave issues about one instruction in 4 to 5 cycles, and that, not the matrix
-// cores, was the limit with 16 x 16 x 32 (6600 cycles a block).  A wave takes
-// 32 keys x 32 rows in QK and 128 latents x 64 rows in PV.
-// 16 and 32 rows are bound by memory.  Eight waves and products of 16 x 16 x
-// 32: a wave takes 16 keys x 16 rows in QK (of a 16-row tile four waves take
-// none) and 64 latents in PV.
+// its keys in blocks of 32.  A workgroup is eight waves, two per SIMD, of two
+// kinds, so that each kind's big operand stays in its registers and one
+// kind's products run beside the other's vector work:
+//   * waves 0 .. 3, rows: S^T = K Q^T of block n + 1 with the queries in
+//     registers (wave w: keys 16 (w & 1) .. + 16, row half w >> 1; of a 16-row
+//     tile waves 0 and 1 alone), then its softmax;
+//   * waves 4 .. 7, latents: O^T += V^T P^T of block n, 128 of the 512 latents
+//     each with the output in registers, and the loads.  bf16 rows come into a
+//     ring of four blocks in LDS by direct global -> LDS loads, three blocks
+//     ahead; INT8 rows as they are, four ahead, converted to bf16 once, two
+//     blocks before their use as V.  The block table's entries come the same
+//     way, two blocks before the loads that need them: nothing waits for memory
+//     but the count of outstanding loads, once a block.
+// The softmax goes against a reference maximum that moves only when a row's
+// maximum passes it by 2^8, so that the output is seldom rescaled; sums, output
+// and references are fp32.  P goes through LDS as bf16; V is read from the rows
+// that served as K, with transposing reads.  Two barriers a block: after the
+// row maxima (halves of the keys are in two waves) and after P.
 // Few tiles (decode): the blocks of all tiles are laid end to end and cut
 // into equal runs, one per workgroup; a tile that several workgroups share
 // leaves fp32 partials that the merge kernel joins.  Many tiles: one
 // workgroup each, longest first.
+#include <math.h>
+
 #include <type_traits>
 
 #include "glm53_common.h"
@@ -44,7 +44,7 @@ namespace {
 
 constexpr int kLatent = 512;
 constexpr int kRope = 64;
-constexpr int kKeys = 64;           // keys per block
+constexpr int kKeys = 32;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;       // how far (log2) a row's maximum may pass the reference
@@ -61,12 +61,15 @@ struct ChunkArgs {
   int64_t bt_stride;
   int max_blocks;
   int block_size;
+  uint32_t div_mul;   // position / block_size by multiplication (divide())
+  int div_sh1, div_sh2;
   int num_reqs;
   int first_step;  // of a binary search over the requests: the largest power of two below num_reqs, or 0
   int total_q;
   int heads;
   int num_tiles;   // bound: tile indexes are below it
   float scale_log2;
+  float masked;    // -inf over the scale's sign: a masked logit before its scale
   uint16_t* out;
   int64_t so_t, so_h;
   int out_align16; // out rows 16-byte aligned (else 8)
@@ -76,36 +79,51 @@ struct ChunkArgs {
   int2* shares;    // [num_tiles]: first and last workgroup of a shared tile, or -1
 };
 
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kHalf = 4;                  // waves of a kind
+constexpr int kOwn = kKeys / kHalf;       // rows of a block that a latent wave brings in
+
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
+// Products of PV: 32 latents x 32 rows x 16 keys, or 16 x 16 x 32 of a 16-row tile.
 template <int kTM>
 struct ChunkShape {
-  static constexpr bool kBig = kTM == 64;           // products of 32 x 32 x 16
-  static constexpr int kWaves = kBig ? 4 : 8;
-  static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kOwn = kKeys / kWaves;       // rows of a block that a wave brings in
+  static constexpr bool kBig = kTM >= 32;
 };
 
-template <int kTM>
+template <int kTM, bool kInt8>
 struct __attribute__((aligned(16))) ChunkShared {
-  struct __attribute__((aligned(16))) Block {
+  static constexpr int kBufs = kInt8 ? 3 : 4;
+  struct __attribute__((aligned(16))) Bf16Block {
     uint8_t lat[kKeys][2 * kLatent];   // chunk c of 16 bytes of row k at chunk c ^ swizzle(k)
     uint8_t rope[kKeys][2 * kRope];
-  } kv[2];
-  uint8_t p[kTM][2 * kKeys];           // P, chunk c of row r at c ^ (r % 8), keys in the order of the V operand
-  float red[4][kTM];                   // per key group: maxima; at the end the sums
-  float ref[kTM];                      // alpha when the reference moves, at the end the reference
-  float scl[2][kKeys];                 // INT8 rows' scales
-  uint64_t have[2];                    // bit k: key k of the block has a row
+  };
+  struct __attribute__((aligned(16))) Int8Block {
+    uint8_t lat[kKeys][2 * kLatent];
+  };
+  std::conditional_t<kInt8, Int8Block, Bf16Block> kv[kBufs];
+  uint8_t raw[kInt8 ? 3 : 0][kKeys][kLatent];   // INT8 rows as they are in the cache
+  float raw_scale[kInt8 ? 3 : 0][kKeys];
+  float scl[kInt8 ? 3 : 0][kKeys];              // the scales, 0 for a key without a row
+  uint8_t p[2][kTM][2 * kKeys];        // P, chunk c of 16 bytes of row r at c ^ (r / 2 % 4)
+  int32_t page[8][kKeys];              // block table entries of the coming blocks
+  float red[2][kTM];                   // per key half: maxima; at the end the sums
+  float alpha[2][kTM];                 // what a block's new references scale the output with; at the end the references
   int ends[kMaxSplitTiles];            // blocks up to and with each tile
   int reqs[kMaxSplitTiles];
-  int sums[8];
-  int flag[2];                         // some row's maximum passed its reference
-  int first;
+  uint8_t have[4][kHalf];              // bit j of byte y: key 8 y + j of the block has a row
+  int flag[2];                         // some reference moved
+  int sums[kWaves];
+  int first, first_t0, first_n, first_len;   // the first tile and its request
 };
 
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// At most n loads that this wave sent are still on their way.
+template <int n>
+__device__ __forceinline__ void loads_left() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
@@ -113,7 +131,7 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 
 // 16 bytes per lane from base + off to LDS at dst + 16 * lane.  Written in asm
 // so that the compiler does not wait for it before other LDS reads;
-// loads_done() and a barrier come before the first read of what it brings.
+// loads_left() and a barrier come before the first read of what it brings.
 // (m0 needs a wait state before its use, an SGPR from v_readlane five.  The
 // compiler keeps m0 out of clobber lists and sets it before each use of its
 // own; nothing else here uses it.)
@@ -123,6 +141,10 @@ __device__ __forceinline__ void load_lds16(uint32_t dst, const uint8_t* base, ui
 }
 __device__ __forceinline__ void load_lds16_at(uint32_t dst, const uint8_t* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(p) : "memory");
+}
+
+__device__ __forceinline__ void load_lds4_at(uint32_t dst, const void* p) {   // 4 bytes per lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(p) : "memory");
 }
 
 // Swizzle of a row's 16-byte chunks (on the low three bits of the chunk's
@@ -153,15 +175,16 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Eight INT8 codes as eight bf16 (exact): code + 128 by the byte conversions,
-// which run at the full rate (the signed conversion does at a quarter of it).
+// Eight INT8 codes as eight bf16 (exact): 12 instructions, all at the full rate.
 __device__ __forceinline__ uint4 codes_to_bf16(uint2 v) {
   uint32_t o[4];
-  const uint32_t w[2] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u};
+  const uint32_t w[2] = {v.x, v.y};
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const float f0 = static_cast<float>(w[k] & 0xffu) - 128.f, f1 = static_cast<float>(w[k] >> 8 & 0xffu) - 128.f;
-    const float f2 = static_cast<float>(w[k] >> 16 & 0xffu) - 128.f, f3 = static_cast<float>(w[k] >> 24) - 128.f;
+    const int32_t x = static_cast<int32_t>(w[k]);
+    const float f0 = static_cast<float>((x << 24) >> 24), f1 = static_cast<float>((x << 16) >> 24);
+    const float f2 = static_cast<float>((x << 8) >> 24), f3 = static_cast<float>(x >> 24);
+    // small whole numbers: the bf16 is the high half of the fp32
     o[2 * k] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
     o[2 * k + 1] = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302u);
   }
@@ -174,24 +197,6 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
   return w;
 }
-
-// One K-step's product of 32 keys and 32 rows, the queries in accumulation
-// registers; with kFirst the sum starts at 0.  In asm because the compiler,
-// with most of a lane's 512 registers in use, otherwise copies the queries to
-// vector registers before the products.  The two wait states before the
-// product are what a vector instruction that wrote one of its operands needs;
-// nothing but these products writes s, and product_done() comes before its
-// first other use.
-template <bool kFirst>
-__device__ __forceinline__ void product(f32x16& s, bf16x8 k, bf16x8 q) {
-  if constexpr (kFirst)
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "a"(q));
-  else
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "a"(q));
-}
-// Wait states between a product and a vector instruction that reads it (19
-// for the longest products; 24 here).
-__device__ __forceinline__ void product_done(f32x16& s) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s)); }
 
 // What a request's tokens and keys are, from values that may be anything:
 // token ranges are clipped to the queries there are, lengths to the table.
@@ -232,30 +237,31 @@ __device__ __forceinline__ LateArgs* late_args() {
   return (LateArgs*)p;
 }
 
+__device__ __forceinline__ int divide(uint32_t n, uint32_t mul, int sh1, int sh2) {
+  const uint32_t t = __umulhi(mul, n);
+  return static_cast<int>((t + ((n - t) >> sh1)) >> sh2);
+}
+
 template <int kTM, bool kInt8, bool kSplit>
-__global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
-  using Shape = ChunkShape<kTM>;
-  constexpr bool kBig = Shape::kBig;
-  constexpr int kWaves = Shape::kWaves, kThreads = Shape::kThreads, kOwn = Shape::kOwn;
-  constexpr int kRowSize = kBig ? 32 : 16;         // rows and latents of a product
-  constexpr int kRT = kTM / kRowSize;              // row tiles
-  constexpr int kLT = kLatent / kRowSize / kWaves; // PV: latent tiles of a wave
-  constexpr int kDepth = kBig ? 16 : 32;           // K-step of a product
-  constexpr int kSteps = (kInt8 ? kLatent : kLatent + kRope) / kDepth;
+__global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
+  using Shared = ChunkShared<kTM, kInt8>;
+  constexpr bool kBig = ChunkShape<kTM>::kBig;
+  constexpr int kRQ = kTM == 64 ? 2 : 1;           // QK: row tiles (of 16) of a wave
+  constexpr int kSteps = kInt8 ? 16 : 18;          // QK: K-steps of 32
+  constexpr int kSize = kBig ? 32 : 16;            // PV: rows and latents of a product
+  constexpr int kRT = kTM / kSize, kLT = 128 / kSize;   // PV: row and latent tiles of a wave
+  constexpr int kDepth = kBig ? 16 : 32;           // PV: keys of a product
   constexpr int kPvSteps = kLT * kKeys / kDepth;
-  constexpr int kLoads = kOwn + (kInt8 ? 0 : kOwn / 8);   // loads a wave sends per block
+  constexpr int kBufs = Shared::kBufs;
+  constexpr int kAhead = kInt8 ? 4 : 3;            // blocks between a row's load and its use as V
+  constexpr int kEarly = kAhead - 1;               // blocks that are asked for before the loop
+  constexpr int kLoads = kInt8 ? 6 : 10;           // loads a latent wave sends per block
   using Acc = std::conditional_t<kBig, f32x16, f32x4>;
   constexpr int kAcc = kBig ? 16 : 4;
-  __shared__ ChunkShared<kTM> sh;
+  __shared__ Shared sh;
 
   const int w = uniform(threadIdx.x >> 6);
   int lane = threadIdx.x & 63;
-  // What depends on the lane alone would be kept in registers across the
-  // block loop; forget() makes the compiler derive it anew from the lane.
-  auto forget = [&]() { asm volatile("" : "+v"(lane)); };
-  // QK: the wave's key group (32 or 16 keys) and row tile
-  const int kg = kBig ? w & 1 : w & 3, rh = kBig ? w >> 1 : w >> 2;
-  const bool takes_rows = rh < kRT;
   const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.block_size;
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
@@ -264,6 +270,7 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
   if (kSplit) {
     constexpr int kTiles = kMaxSplitTiles / kThreads;   // tiles of a thread
     int units[kTiles], req[kTiles], sum = 0;
+    Request of[kTiles];
     int* cu_s = reinterpret_cast<int*>(&sh.kv[0]);      // cu, then lens
     for (int r = threadIdx.x; r <= a.num_reqs; r += kThreads) cu_s[r] = min(max(a.cu[r], 0), a.total_q);
     int* len_s = cu_s + kMaxSplitTiles + 16;
@@ -280,6 +287,7 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
       const Request rq = request_of(cu_s[at], cu_s[at + 1], len_s[at], a.total_q);
       const int row0 = (t - first_tile<kTM>(rq.t0, a.heads, at)) * kTM;
       req[k] = at;
+      of[k] = rq;
       units[k] = 0;
       if (t < a.num_tiles && row0 >= 0 && row0 < rq.n * a.heads)
         units[k] = max(1, last_key<kTM>(rq, row0, a.heads, max_pos) / kKeys + 1);
@@ -315,7 +323,8 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
 #pragma unroll
     for (int k = 0; k < kTiles; k++) {
       const int t = static_cast<int>(threadIdx.x) * kTiles + k;
-      if (end <= lo && lo < end + units[k]) sh.first = t;
+      if (end <= lo && lo < end + units[k])
+        sh.first = t, sh.first_t0 = of[k].t0, sh.first_n = of[k].n, sh.first_len = of[k].len;
       end += units[k];
       sh.ends[t] = end;
       sh.reqs[t] = req[k];
@@ -328,8 +337,9 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
   }
 
   for (;; tile++) {
-    // ---- the tile: its request, its rows, its blocks [b0, b1)
-    int r, b0 = 0, b1 = 0, start = 0, units = 0;
+    asm volatile("" : "+v"(lane));   // nothing that depends on the lane alone is kept from tile to tile
+    // ---- the tile: its request, its rows, its blocks [b0, b0 + count)
+    int r, b0 = 0, count = 0, start = 0, units = 0;
     if (kSplit) {
       if (tile >= kMaxSplitTiles) return;
       start = tile ? uniform(sh.ends[tile - 1]) : 0;
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
       if (units == 0) continue;
       r = uniform(sh.reqs[tile]);
       b0 = max(lo - start, 0);
-      b1 = min(hi - start, units);
+      count = min(hi - start, units) - b0;
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
       int begun = 0;
@@ -354,104 +364,34 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
       for (int i = 0; i < kWaves; i++) r += sh.sums[i];
       r = uniform(max(r, 0));
     }
-    const Request rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
+    Request rq;
+    if (kSplit && tile == uniform(sh.first))
+      rq = {uniform(sh.first_t0), uniform(sh.first_n), uniform(sh.first_len)};
+    else
+      rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
     const int last = last_key<kTM>(rq, row0, a.heads, max_pos);
     if (!kSplit)
-      b1 = last >= 0 ? last / kKeys + 1 : 0;
+      count = last >= 0 ? last / kKeys + 1 : 0;
     else if (last < 0)
-      b1 = b0;   // nothing to see: its one unit writes the zeros
+      count = 0;   // nothing to see: its one unit writes the zeros
     // the least of the rows' last positions: keys past it are masked for some row
     const int64_t least64 = static_cast<int64_t>(rq.len) - rq.n + row0 / a.heads;
     const int least = static_cast<int>(least64 < -1 ? -1 : least64 < last ? least64 : last);
 
     if (kSplit) wg_barrier();   // LDS is free (the tile before, the scan)
 
-    // ---- bringing blocks in.  Wave w brings in the rows of keys kOwn w ... .
-    // Lane c (of each kOwn) looks up key kOwn w + c: its page in the table, one
-    // block ahead of its use, then its row's address.  A key past the last one
-    // seen, or whose page is not in the table or the cache, has no row: the
-    // cache's first is read in its place and zeroed.  After the last block
-    // there are no rows, and the loads bring nothing that is used.
-    uint2 codes[kInt8 ? kOwn : 1];
-    float scale = 0.f;
-    int pos = b0 * kKeys + kOwn * w + (lane & (kOwn - 1));   // of the block that `page` is for
-    int pg = pos / a.block_size, in_page = pos - pg * a.block_size, page = -1;
-    const int step_pg = kKeys / a.block_size, step_in = kKeys - step_pg * a.block_size;
-    const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
-    auto look_up = [&](int b) { page = b < b1 && pos <= last && pg < a.max_blocks ? bt[pg] : -1; };
-    auto advance = [&]() {
-      pos += kKeys;
-      pg += step_pg;
-      in_page += step_in;
-      if (in_page >= a.block_size) in_page -= a.block_size, pg++;
-    };
-    uint32_t row_lo = 0, row_hi = 0, mine = 0;   // addresses; bit j: this wave's row j is there
-    constexpr uint32_t kAll = (1u << kOwn) - 1;
-    auto address = [&](int b) {
-      const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
-      mine = static_cast<uint32_t>(__ballot(ok)) & kAll;
-      const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
-                          (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
-      row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
-      if (lane == 0) {
-        if constexpr (kBig)
-          reinterpret_cast<uint16_t*>(&sh.have[b & 1])[w] = static_cast<uint16_t>(mine);
-        else
-          reinterpret_cast<uint8_t*>(&sh.have[b & 1])[w] = static_cast<uint8_t>(mine);
-      }
-    };
-    // load j of kLoads of block b
-    auto bring = [&](int b, int j) {
-      auto& blk = sh.kv[b & 1];
-      if (j < kOwn) {
-        const uint64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, j)) |
-                            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, j))) << 32;
-        const uint8_t* row = reinterpret_cast<const uint8_t*>(at);
-        if constexpr (kInt8)
-          codes[j] = *reinterpret_cast<const uint2*>(row + 8 * lane);
-        else
-          load_lds16(lds_offset(blk.lat[kOwn * w + j]), row, (16 * lane) ^ (16 * swizzle(j)));
-      } else if constexpr (!kInt8) {
-        const int key = 8 * (j - kOwn) + (lane >> 3);
-        const uint64_t at = static_cast<uint32_t>(__shfl(static_cast<int>(row_lo), key)) |
-                            static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row_hi), key))) << 32;
-        load_lds16_at(lds_offset(blk.rope[kOwn * w + 8 * (j - kOwn)]),
-                      reinterpret_cast<const uint8_t*>(at) + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(key)));
-      }
-      if (kInt8 && j == kOwn - 1)
-        scale = *reinterpret_cast<const float*>((row_lo | static_cast<uint64_t>(row_hi) << 32) + kLatent);
-    };
-    // INT8: row j of the wave's rows of block b as bf16 into LDS (0 without a row)
-    auto put_row = [&](int b, int j) {
-      if constexpr (kInt8) {
-        const uint32_t keep = 0u - (mine >> j & 1);
-        *reinterpret_cast<uint4*>(&sh.kv[b & 1].lat[kOwn * w + j][(16 * lane) ^ (16 * swizzle(j))]) =
-            codes_to_bf16(make_uint2(codes[j].x & keep, codes[j].y & keep));
-        if (j == kOwn - 1 && lane < kOwn) sh.scl[b & 1][kOwn * w + lane] = mine >> lane & 1 ? scale : 0.f;
-      }
-    };
+    const int g = lane >> 4, c = lane & 15;
+    LateArgs* e = late_args();
 
-    if (b0 < b1) {
-      look_up(b0);
-      address(b0);
-      advance();
-#pragma unroll
-      for (int j = 0; j < kLoads; j++) bring(b0, j);
-      look_up(b0 + 1);
-    }
-
-    // ---- the queries (rows past the last: the last, not stored).  Several
-    // waves need each, so they come through LDS once, in the buffer that the
-    // second block will take, laid out like keys: wave w brings in every
-    // kWaves-th row.
-    bf16x8 qf[kSteps];
-    {
-      auto& qs = sh.kv[(b0 + 1) & 1];
+    // The queries come through LDS, laid out like keys, in the ring's buffers
+    // that the first blocks leave: wave w brings in every eighth row.
+    constexpr int kQBuf = kInt8 ? 1 : 2;
+    auto bring_queries = [&]() {
       constexpr int kMine = kTM / kWaves;
-      const int row = min(row0 + kWaves * min(lane & 15, kMine - 1) + w, rows - 1);
+      const int row = min(row0 + kWaves * min(c, kMine - 1) + w, rows - 1);   // (rows past the last: the last, not stored)
       const int tok = row / a.heads, head = row - tok * a.heads;
       const uint64_t at = reinterpret_cast<uint64_t>(a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t +
                                                      static_cast<int64_t>(head) * a.sq_h);
@@ -462,316 +402,461 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
             static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, j)) |
             static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, j))) << 32);
         const int key = kWaves * j + w;
-        load_lds16(lds_offset(qs.lat[key]), from, 16 * (lane ^ swizzle(key)));
+        auto& qs = sh.kv[kQBuf + (key >> 5)];
+        load_lds16(lds_offset(qs.lat[key & 31]), from, 16 * (lane ^ swizzle(key)));
         if constexpr (!kInt8) {
-          if (lane < 8) load_lds16(lds_offset(qs.rope[key]), from, 2 * kLatent + 16 * (lane ^ swizzle(key)));
+          if (lane < 8) load_lds16(lds_offset(qs.rope[key & 31]), from, 2 * kLatent + 16 * (lane ^ swizzle(key)));
         }
       }
-      loads_done();   // the queries, and the first block's rows
-      wg_barrier();
-      const int key = kRowSize * (takes_rows ? rh : 0) + (lane & (kRowSize - 1)), sw = swizzle(lane), part = lane / kRowSize;
-      constexpr int kChunks = kDepth / 8;   // 16-byte chunks of a K-step
-#pragma unroll
-      for (int st = 0; st < kSteps; st++) {
-        const int chunk = kChunks * st;     // + part
-        const uint8_t* from = chunk < 64 ? qs.lat[key] + 16 * (((chunk & 7) + part) ^ sw) + 128 * (chunk >> 3)
-                                         : qs.rope[key] + 16 * ((chunk - 64 + part) ^ sw);
-        qf[st] = *reinterpret_cast<const bf16x8*>(from);
-      }
-    }
-    Acc acc[kLT][kRT];
-#pragma unroll
-    for (int i = 0; i < kLT; i++)
-#pragma unroll
-      for (int j = 0; j < kRT; j++)
-#pragma unroll
-        for (int e = 0; e < kAcc; e++) acc[i][j][e] = 0.f;
-    // the reference maximum (log2) of this lane's row, from the least number on: every other logit passes it
-    float ref = -3.4028234663852886e38f, sum = 0.f;
-    if (b0 < b1) {
-#pragma unroll
-      for (int j = 0; j < kOwn; j++) put_row(b0, j);
-    }
-    if (threadIdx.x == 0) sh.flag[0] = sh.flag[1] = 0;
+    };
 
-    for (int b = b0; b < b1; b++) {
-      loads_done();   // this wave's rows of block b
-      auto& blk = sh.kv[b & 1];
-      if (!kInt8 && mine != kAll) {
-        for (int j = 0; j < kOwn; j++)
-          if (!(mine >> j & 1)) {
-            *reinterpret_cast<uint4*>(&blk.lat[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
-            if (lane < 8) *reinterpret_cast<uint4*>(&blk.rope[kOwn * w + j][16 * lane]) = make_uint4(0, 0, 0, 0);
-          }
-      }
-      wg_barrier();   // every wave's rows are there; nobody reads the other buffer, P or the maxima any more
-      forget();
-      if (w == 0 && lane == 0) sh.flag[(b + 1) & 1] = 0;
-      const uint64_t have_v = sh.have[b & 1];
-      address(b + 1);
-
-      // ---- S^T = K Q^T: the wave's keys, one row a lane.  Each K-step's
-      // operand is read some steps before its product; between the steps the
-      // next block's rows are asked for - all of them here where memory bounds
-      // the loop, and spread over the block where the products do: sent at
-      // once they fill the CU's miss queue and hold up the products behind.
-      constexpr int kInQk = kBig && !kInt8 ? 12 : kLoads, kInSm = kBig && !kInt8 ? 3 : 0;
-      Acc s;
-      if (takes_rows) {
-        constexpr int kRead = kBig ? 6 : 5, kChunks = kDepth / 8;
-        const int key = kRowSize * kg + (lane & (kRowSize - 1)), sw = swizzle(lane), part = lane / kRowSize;
-        const uint8_t* base[8 / kChunks];
+    if (w < kHalf) {
+      // ================ rows: QK and softmax, a block ahead of PV
+      const int kh = w & 1, rh = w >> 1;
+      const bool takes_rows = rh * 16 * kRQ < kTM;
+      bring_queries();
+      loads_left<0>();
+      wg_barrier();   // the queries, the first blocks' rows
+      bf16x8 qf[kRQ][kSteps];
 #pragma unroll
-        for (int i = 0; i < 8 / kChunks; i++) base[i] = blk.lat[key] + 16 * ((kChunks * i + part) ^ sw);
-        const uint8_t* rope = blk.rope[key];
-        auto operand = [&](int st) {
-          const int chunk = kChunks * st;
-          return *reinterpret_cast<const bf16x8*>(chunk < 64 ? base[st % (8 / kChunks)] + 128 * (chunk >> 3)
-                                                             : rope + 16 * ((chunk - 64 + part) ^ sw));
-        };
-        bf16x8 k[kSteps];
-        Acc odd;
-#pragma unroll
-        for (int e = 0; e < kAcc; e++) odd[e] = 0.f;
-#pragma unroll
-        for (int st = 0; st < kRead; st++) k[st] = operand(st);
+      for (int rt = 0; rt < kRQ; rt++) {
+        const int key = 16 * (takes_rows ? rh * kRQ + rt : 0) + c, sw = swizzle(c);
+        const auto& qs = sh.kv[kQBuf + (key >> 5)];
 #pragma unroll
         for (int st = 0; st < kSteps; st++) {
-          if (st + kRead < kSteps) k[st + kRead] = operand(st + kRead);
-          if constexpr (kBig) {
-            if (st == 0)
-              product<true>(s, k[st], qf[st]);
-            else
-              product<false>(s, k[st], qf[st]);
-            if (kInt8 ? st % 2 == 0 : st % 3 == 0) bring(b + 1, kInt8 ? st / 2 : st / 3);
-          } else {   // two sums, so that a product does not wait for the one before it
-            if (st == 0)
-#pragma unroll
-              for (int e = 0; e < kAcc; e++) s[e] = 0.f;
-            if (st & 1)
-              odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[st], odd, 0, 0, 0);
-            else
-              s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[st], s, 0, 0, 0);
-            if (st < kLoads) bring(b + 1, st);
+          const uint8_t* from = qs.lat[key & 31] + 16 * ((4 * (st & 1) + g) ^ sw) + 128 * (st >> 1);
+          if constexpr (!kInt8) {
+            if (st >= 16) from = qs.rope[key & 31] + 16 * ((4 * (st - 16) + g) ^ sw);
           }
-          __builtin_amdgcn_sched_barrier(0);
+          qf[rt][st] = *reinterpret_cast<const bf16x8*>(from);
         }
-        if constexpr (kBig) {
-          product_done(s);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kAcc; e++) s[e] += odd[e];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kLoads; j++) bring(b + 1, j);
       }
-      forget();
-
-      // ---- softmax.  Element e of a lane is key key_of(e) of the block, its
-      // row c of row tile rh.
-      const int part = lane / kRowSize, c = lane & (kRowSize - 1);
-      auto key_of = [&](int e) { return kRowSize * kg + (kBig ? 8 * (e >> 2) + 4 * part + (e & 3) : 4 * part + e); };
-      float weights = 0.f;
-      float ksv[kInt8 ? kAcc : 1];
-      auto put_p = [&]() {
-        float p[kAcc];
+      wg_barrier();   // the queries have been read
+      // the reference maxima (log2) of this lane's rows, from the least number on: every other logit passes it
+      float ref[kRQ], sum[kRQ];
 #pragma unroll
-        for (int e = 0; e < kAcc; e++) p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
-        float t[kAcc / 4];
+      for (int rt = 0; rt < kRQ; rt++) ref[rt] = -3.4028234663852886e38f, sum[rt] = 0.f;
+      int buf = 0;
+      for (int n = 0; n < count; n++) {
+        // ---- S^T = K Q^T: keys 16 kh + 4 g + i of block n, rows c.  Each
+        // K-step's operand is read some steps before its products.
+        f32x4 s[kRQ];
+        float ksv[4] = {1.f, 1.f, 1.f, 1.f};
+        if (takes_rows) {
+          constexpr int kRead = 6;
+          const int key = 16 * kh + c, sw = swizzle(c);
+          const auto& blk = sh.kv[buf];
+          const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
+          const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
+          auto operand = [&](int st) {
+            const uint8_t* from = (st & 1 ? odd : even) + 128 * (st >> 1);
+            if constexpr (!kInt8) {
+              if (st >= 16) from = blk.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
+            }
+            return *reinterpret_cast<const bf16x8*>(from);
+          };
+          const uint32_t have = static_cast<uint32_t>(*reinterpret_cast<const int*>(sh.have[n & 3]));
+          if constexpr (kInt8) {
+            const float4 v = *reinterpret_cast<const float4*>(&sh.scl[buf][16 * kh + 4 * g]);
+            ksv[0] = v.x, ksv[1] = v.y, ksv[2] = v.z, ksv[3] = v.w;
+          }
+          // two sums with one row tile, so that a product does not wait for the one before it
+          constexpr int kSums = kRQ == 1 ? 2 : 1;
+          f32x4 t[kRQ][kSums];
 #pragma unroll
-        for (int e = 0; e < kAcc; e += 4) t[e / 4] = (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
-        weights = kBig ? (t[0] + t[1 % (kAcc / 4)]) + (t[2 % (kAcc / 4)] + t[3 % (kAcc / 4)]) : t[0];
-        if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
+          for (int rt = 0; rt < kRQ; rt++)
 #pragma unroll
-          for (int e = 0; e < kAcc; e++) p[e] *= ksv[e];
+            for (int u = 0; u < kSums; u++) t[rt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          bf16x8 k[kSteps];
+#pragma unroll
+          for (int st = 0; st < kRead; st++) k[st] = operand(st);
+#pragma unroll
+          for (int st = 0; st < kSteps; st++) {
+            if (st + kRead < kSteps) k[st + kRead] = operand(st + kRead);
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++)
+              t[rt][st % kSums] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], t[rt][st % kSums], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int rt = 0; rt < kRQ; rt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              s[rt][i] = kSums == 1 ? t[rt][0][i] : t[rt][0][i] + t[rt][kSums - 1][i];
+              // bf16: the logits keep their scale until their weights are taken
+              if constexpr (kInt8) s[rt][i] *= a.scale_log2 * ksv[i];
+            }
+          if (uniform(static_cast<int>(have)) != -1 || (b0 + n + 1) * kKeys - 1 > least) {
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++) {
+              const int row = min(row0 + 16 * (rh * kRQ + rt) + c, rows - 1);
+              const int64_t see = static_cast<int64_t>(rq.len) - rq.n + row / a.heads;
+              const int limit = static_cast<int>(see < last ? see < -1 ? -1 : see : last) - (b0 + n) * kKeys;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int key = 16 * kh + 4 * g + i;
+                if (key > limit || !(have >> key & 1)) s[rt][i] = kInt8 ? -INFINITY : a.masked;
+              }
+            }
+          }
+          if constexpr (kInt8) {
+            // a scale that is not a number has made its logits so; where it is
+            // masked, the weight 0 has to stay 0
+#pragma unroll
+            for (int i = 0; i < 4; i++) ksv[i] = fabsf(ksv[i]) < INFINITY ? ksv[i] : 0.f;
+          }
+#pragma unroll
+          for (int rt = 0; rt < kRQ; rt++) {
+            float top;
+            if (kInt8 || a.scale_log2 >= 0.f)
+              top = fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]));
+            else
+              top = fminf(fminf(s[rt][0], s[rt][1]), fminf(s[rt][2], s[rt][3]));
+            if constexpr (!kInt8) top *= a.scale_log2;
+            top = quad_max(top);
+            if (lane < 16) sh.red[kh][16 * (rh * kRQ + rt) + c] = top;
+          }
         }
-        // P is rounded to bf16 (like the output, 2^-9 of each weight on the
-        // average); the sum keeps the unrounded weights.  Chunk of 8 keys and
-        // half: with the small products the operand's keys of each 32 are
-        // 4 g + i and 16 + 4 g + i.
-        uint8_t* row = sh.p[kRowSize * rh + c];
+        wg_barrier();   // the maxima
+        if (takes_rows) {
+          // ---- softmax: a row's reference moves where its maximum passed it
+          // by 2^8; both waves of a row decide alike
+          bool moved = false;
+          float scaled[kRQ];
 #pragma unroll
-        for (int e = 0; e < kAcc; e += 4) {
-          const int chunk = kBig ? 4 * kg + e / 4 : 4 * (kg >> 1) + part, half = kBig ? part : kg & 1;
-          *reinterpret_cast<uint2*>(row + 16 * (chunk ^ (c & 7)) + 8 * half) =
-              make_uint2(pack_bf16x2(p[e], p[e + 1]), pack_bf16x2(p[e + 2], p[e + 3]));
+          for (int rt = 0; rt < kRQ; rt++) {
+            const int row = 16 * (rh * kRQ + rt) + c;
+            const float m = fmaxf(sh.red[0][row], sh.red[1][row]);
+            scaled[rt] = ref[rt];
+            if (m > ref[rt] + kSlack) ref[rt] = m, moved = true;
+          }
+          if (__ballot(moved)) {
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++) {
+              const float alpha = __builtin_amdgcn_exp2f(scaled[rt] - ref[rt]);
+              sum[rt] *= alpha;
+              if (kh == 0 && lane < 16) sh.alpha[n & 1][16 * (rh * kRQ + rt) + c] = alpha;
+            }
+            if (lane == 0) sh.flag[n & 1] = 1;
+          } else if (kh == 0 && lane < 16) {   // the other row half's may have moved
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++) sh.alpha[n & 1][16 * (rh * kRQ + rt) + c] = 1.f;
+          }
+#pragma unroll
+          for (int rt = 0; rt < kRQ; rt++) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              p[i] = __builtin_amdgcn_exp2f(kInt8 ? s[rt][i] - ref[rt] : __builtin_fmaf(s[rt][i], a.scale_log2, -ref[rt]));
+            sum[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+            if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
+#pragma unroll
+              for (int i = 0; i < 4; i++) p[i] *= ksv[i];
+            }
+            // P is rounded to bf16 (like the output, 2^-9 of each weight on
+            // the average); the sum keeps the unrounded weights.  With the
+            // small products of PV the operand's keys are 4 g + i, 16 + 4 g + i.
+            const int chunk = kBig ? 2 * kh + (g >> 1) : g, half = kBig ? g & 1 : kh;
+            *reinterpret_cast<uint2*>(sh.p[n & 1][16 * (rh * kRQ + rt) + c] + 16 * (chunk ^ (c >> 1 & 3)) + 8 * half) =
+                make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
+          }
+        }
+        wg_barrier();   // P
+        buf = buf + 1 < kBufs ? buf + 1 : 0;
+      }
+      if (count) {   // PV of the last block
+        wg_barrier();
+        wg_barrier();
+      }
+      wg_barrier();   // PV has read P and the references' changes for the last time
+      if (takes_rows) {
+#pragma unroll
+        for (int rt = 0; rt < kRQ; rt++) {
+          const float l = quad_sum(sum[rt]);
+          const int row = 16 * (rh * kRQ + rt) + c;
+          if (lane < 16) sh.red[kh][row] = l;
+          if (kh == 0 && lane < 16) sh.alpha[0][row] = ref[rt];
+        }
+      }
+      wg_barrier();   // the sums
+    } else {
+      // ================ latents: loads, PV
+      const int y = w - kHalf;
+      // ---- bringing blocks in, counted from the first (block n has the
+      // positions 32 (b0 + n) + [0, 32)).  Wave y brings in rows 8 y .. 8 y + 7;
+      // lane l looks after row 8 y + l / 8: its page from the table, then its
+      // address.  A key past the last one seen, or whose page is not in the
+      // table or the cache, has no row: the cache's first is read in its place
+      // and zeroed, so that every wave sends kLoads loads a block, also for
+      // blocks past the end.
+      const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
+      auto look_up = [&](int n) {       // the block table's entries for block n, by every wave
+        const int pos = min((b0 + n) * kKeys + (lane & 31), last);
+        const int pg = divide(pos, a.div_mul, a.div_sh1, a.div_sh2);
+        if (lane < 32) load_lds4_at(lds_offset(sh.page[n & 7]), bt + pg);
+      };
+      uint32_t row_lo = 0, row_hi = 0, masks = 0;   // masks: a byte per block on its way, this wave's rows
+      auto address = [&](int n) {
+        const int key = kOwn * y + (lane >> 3), pos = (b0 + n) * kKeys + key;
+        const int page = sh.page[n & 7][key];
+        const int in_page = pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size;
+        const bool ok = n < count && pos <= last && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
+        const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
+                            (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
+        row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
+        // bit 8 j of the ballot to bit j
+        const uint32_t mask = static_cast<uint32_t>(((__ballot(ok) & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+        if (lane == 0) sh.have[n & 3][y] = static_cast<uint8_t>(mask);
+        return mask;
+      };
+      auto row_of = [&](int j) {        // uniform: row j of the wave's
+        return reinterpret_cast<const uint8_t*>(
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, 8 * j)) |
+            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, 8 * j))) << 32);
+      };
+      auto row_at = [&](int j) {        // per lane
+        return reinterpret_cast<const uint8_t*>(
+            static_cast<uint32_t>(__shfl(static_cast<int>(row_lo), 8 * j)) |
+            static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row_hi), 8 * j))) << 32);
+      };
+      // load j of kLoads - 1 of block n's rows into buffer `to`
+      auto bring = [&](int to, int j) {
+        if constexpr (kInt8) {
+          if (j < 4)
+            load_lds16_at(lds_offset(sh.raw[to][kOwn * y + 2 * j]), row_at(2 * j + (lane >> 5)) + 16 * (lane & 31));
+          else {
+            const uint8_t* row = row_at(lane & 7);
+            if (lane < kOwn) load_lds4_at(lds_offset(&sh.raw_scale[to][kOwn * y]), row + kLatent);
+          }
+        } else {
+          if (j < kOwn) {
+            load_lds16(lds_offset(sh.kv[to].lat[kOwn * y + j]), row_of(j), (16 * lane) ^ (16 * swizzle(j)));
+          } else {
+            const uint8_t* row = reinterpret_cast<const uint8_t*>(row_lo | static_cast<uint64_t>(row_hi) << 32);
+            load_lds16_at(lds_offset(sh.kv[to].rope[kOwn * y]), row + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3)));
+          }
         }
       };
-      if (takes_rows) {
-        const uint64_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v))) |
-                              static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(have_v >> 32)))) << 32;
+      auto zero_rows = [&](int in, uint32_t mask) {   // bf16: rows that are not there, after the loads in their place
+        if constexpr (!kInt8) {
+          for (int j = 0; j < kOwn; j++)
+            if (!(mask >> j & 1)) {
+              *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * y + j][16 * lane]) = make_uint4(0, 0, 0, 0);
+              if (lane < 8) *reinterpret_cast<uint4*>(&sh.kv[in].rope[kOwn * y + j][16 * lane]) = make_uint4(0, 0, 0, 0);
+            }
+        }
+      };
+      // INT8: row j of the wave's from raw block `in` to the bf16 block there (0 without a row)
+      auto convert = [&](int in, int j, uint32_t mask) {
         if constexpr (kInt8) {
-#pragma unroll
-          for (int e = 0; e < kAcc; e += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(&sh.scl[b & 1][key_of(e)]);
-            ksv[e] = v.x, ksv[e + 1] = v.y, ksv[e + 2] = v.z, ksv[e + 3] = v.w;
-          }
+          const uint2 v = *reinterpret_cast<const uint2*>(&sh.raw[in][kOwn * y + j][8 * lane]);
+          const uint32_t keep = 0u - (mask >> j & 1);
+          *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * y + j][(16 * lane) ^ (16 * swizzle(j))]) =
+              codes_to_bf16(make_uint2(v.x & keep, v.y & keep));
+          if (j == 0 && lane < kOwn)
+            sh.scl[in][kOwn * y + lane] = mask >> lane & 1 ? sh.raw_scale[in][kOwn * y + lane] : 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < kAcc; e++) s[e] *= kInt8 ? a.scale_log2 * ksv[kInt8 ? e : 0] : a.scale_log2;
-        if (have != ~0ull || (b + 1) * kKeys - 1 > least) {
-          const int row = min(row0 + kRowSize * rh + c, rows - 1);
-          const int64_t see = static_cast<int64_t>(rq.len) - rq.n + row / a.heads;
-          const int limit = static_cast<int>(see < last ? see < -1 ? -1 : see : last) - b * kKeys;
-#pragma unroll
-          for (int e = 0; e < kAcc; e++) {
-            const int k = key_of(e);
-            if (k > limit || !(have >> k & 1)) s[e] = -INFINITY;
-          }
-        }
-        if constexpr (kInt8) {
-          // a scale that is not a number has made its logits so; where it is
-          // masked, the weight 0 has to stay 0
-#pragma unroll
-          for (int e = 0; e < kAcc; e++) ksv[e] = fabsf(ksv[e]) < INFINITY ? ksv[e] : 0.f;
-        }
-        if (kInSm > 0) bring(b + 1, kInQk);
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < kAcc; e++) top = fmaxf(top, s[e]);
-        top = kBig ? half_max(top) : quad_max(top);
-        if (lane < kRowSize) sh.red[kg][kRowSize * rh + c] = top;
-        if (__ballot(top > ref + kSlack) && lane == 0) sh.flag[b & 1] = 1;
-        if (kInSm > 1) bring(b + 1, kInQk + 1);
-        put_p();
-        if (kInSm > 2) bring(b + 1, kInQk + 2);
-      }
-      advance();
-      look_up(b + 2);
-      wg_barrier();   // P is whole
+      };
 
-      if (uniform(sh.flag[b & 1])) {   // some row's maximum passed its reference: all rows take theirs
-        if (takes_rows) {
-          const int row = kRowSize * rh + c;
-          float m = ref;
+      if (count) {
 #pragma unroll
-          for (int i = 0; i < kKeys / kRowSize; i++) m = fmaxf(m, sh.red[i][row]);
-          const float alpha = __builtin_amdgcn_exp2f(ref - m);
-          ref = m;
-          sum *= alpha;
-          if (kg == 0 && lane < kRowSize) sh.ref[row] = alpha;
-          put_p();
-        }
-        wg_barrier();
+        for (int n = 0; n < kEarly + 2; n++) look_up(n);
+        loads_left<0>();
 #pragma unroll
-        for (int j = 0; j < kRT; j++) {
-          const float alpha = sh.ref[kRowSize * j + c];
+        for (int n = 0; n < kEarly; n++) {
+          masks |= address(n) << (8 * n);
 #pragma unroll
-          for (int i = 0; i < kLT; i++)
-#pragma unroll
-            for (int e = 0; e < kAcc; e++) acc[i][j][e] *= alpha;
+          for (int j = 0; j < kLoads - 1; j++) bring(n, j);
         }
       }
-      sum += weights;
-
-      if constexpr (!kInt8) {
-        // Keys that some row of the tile may not see: 0 * inf would put NaN
-        // into that row.  A row that sees such a key has NaN from its logit.
-        if ((b + 1) * kKeys - 1 > least && least < last) {
-          for (int j = 0; j < kOwn; j++) {
-            uint4* at = reinterpret_cast<uint4*>(&blk.lat[kOwn * w + j][16 * lane]);
-            const uint4 v = *at;
-            *at = make_uint4(finite_bf16x2(v.x), finite_bf16x2(v.y), finite_bf16x2(v.z), finite_bf16x2(v.w));
-          }
-          wg_barrier();
+      bring_queries();
+      loads_left<0>();
+      if (count) {
+        if (kInt8) {
+#pragma unroll
+          for (int j = 0; j < kOwn; j++) convert(0, j, masks);
+        } else {
+          if ((masks & 0xff) != 0xff) zero_rows(0, masks);
         }
+        masks >>= 8;   // of the blocks from 1
       }
-      forget();
+      if (w == kHalf && lane < 2) sh.flag[lane] = 0;
+      wg_barrier();   // the queries, the first block's rows
+      Acc acc[kLT][kRT];
+#pragma unroll
+      for (int i = 0; i < kLT; i++)
+#pragma unroll
+        for (int j = 0; j < kRT; j++)
+#pragma unroll
+          for (int q = 0; q < kAcc; q++) acc[i][j][q] = 0.f;
+      wg_barrier();   // the queries have been read
 
-      // ---- O^T += V^T P^T: the wave's latent tiles, all rows; V's operands are
-      // read some steps ahead.  INT8: a row of the next block is converted
-      // between the steps.
-      {
-        constexpr int kRead = kBig ? 4 : 3, kGroups = kKeys / kDepth;
-        const int g = lane >> 4, c16 = lane & 15;
+      // iteration n: PV of block n (the rows' waves are at block n + 1)
+      int buf = kBufs - 1;   // of block n
+      for (int n = -1; n < count && count; n++) {
+        const int next = buf + 1 < kBufs ? buf + 1 : 0, after = next + 1 < kBufs ? next + 1 : 0;
+        // bf16: block n + 3 comes into the buffer of block n - 1; INT8: block n
+        // + 4 into the raw one of block n + 1 (converted in the iteration
+        // before), and block n + 2 is converted
+        const int into = kInt8 ? next : buf > 0 ? buf - 1 : kBufs - 1;
+        const uint32_t mask = address(n + kAhead);
+        if (n >= 0 && uniform(sh.flag[n & 1])) {
+#pragma unroll
+          for (int j = 0; j < kRT; j++) {
+            const float alpha = sh.alpha[n & 1][kSize * j + (lane & (kSize - 1))];
+#pragma unroll
+            for (int i = 0; i < kLT; i++)
+#pragma unroll
+              for (int q = 0; q < kAcc; q++) acc[i][j][q] *= alpha;
+          }
+        }
+        if constexpr (!kInt8) {
+          // Keys that some row of the tile may not see: 0 * inf would put NaN
+          // into that row.  A row that sees such a key has NaN from its logit.
+          // (This wave's latents of all rows.)
+          if (n >= 0 && (b0 + n + 1) * kKeys - 1 > least && least < last) {
+            for (int j = 0; j < kKeys; j += 4) {
+              uint4* at = reinterpret_cast<uint4*>(&sh.kv[buf].lat[j + g][256 * y + 16 * c]);
+              const uint4 v = *at;
+              *at = make_uint4(finite_bf16x2(v.x), finite_bf16x2(v.y), finite_bf16x2(v.z), finite_bf16x2(v.w));
+            }
+          }
+        }
+
+        // ---- O^T += V^T P^T: V's operands are read some steps ahead; between
+        // the steps come the loads of a later block and the conversion.  In
+        // the iteration before block 0 the weights and the output are zero.
+        constexpr int kRead = 4, kGroups = kKeys / kDepth, kFirst = kPvSteps / 2;
+        const int part = lane / kSize, pr = lane & (kSize - 1), c16 = lane & 15;
         // a transposing read gives a lane its column (latent) of four rows (keys)
         const int tr_row = kBig ? 8 * (lane >> 5) + (c16 >> 2) : 4 * g + (c16 >> 2);
         const int tr_col = (kBig ? 2 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
-        constexpr int kTileChunks = kRowSize / 8, kBases = 8 / kTileChunks;  // the swizzle is on 8 chunks
-        constexpr int kSecond = (kBig ? 4 : 16) * 2 * kLatent;               // rows of the operand's other half
+        constexpr int kTileChunks = kSize / 8, kBases = 8 / kTileChunks;     // the swizzle is on 8 chunks
         const uint8_t* base[kBases][kBig ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < kBases; i++)
 #pragma unroll
           for (int h = 0; h < (kBig ? 2 : 1); h++)
-            base[i][h] = &blk.lat[tr_row + 4 * h][128 * (kLT * kTileChunks * w / 8) +
-                                                  16 * ((kTileChunks * i + tr_col) ^ swizzle(tr_row + 4 * h)) + 8 * (c16 & 1)];
+            base[i][h] = &sh.kv[buf].lat[tr_row + 4 * h][256 * y + 16 * ((kTileChunks * i + tr_col) ^ swizzle(tr_row + 4 * h)) +
+                                                         8 * (c16 & 1)];
         auto operand = [&](int u) {
           const int i = u % kLT, t = u / kLT;   // latent tile, keys
           const int off = 128 * (i / kBases) + kDepth * t * 2 * kLatent;
           const uint8_t* p0 = base[i % kBases][0] + off;
-          const uint8_t* p1 = kBig ? base[i % kBases][kBig ? 1 : 0] + off : p0 + kSecond;
+          const uint8_t* p1 = kBig ? base[i % kBases][kBig ? 1 : 0] + off : p0 + 16 * 2 * kLatent;
           const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p0)));
           const i32x2 v1 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p1)));
           return __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
         };
-        auto weights_of = [&](int t, int j) {
-          const int chunk = kDepth / 8 * t + part;
-          return *reinterpret_cast<const bf16x8*>(sh.p[kRowSize * j + c] + 16 * (chunk ^ (c & 7)));
-        };
         bf16x8 pb[kGroups][kRT], v[kPvSteps];
+        if (n >= 0) {
 #pragma unroll
-        for (int j = 0; j < kRT; j++) pb[0][j] = weights_of(0, j);
+          for (int t = 0; t < kGroups; t++)
 #pragma unroll
-        for (int u = 0; u < kRead; u++) v[u] = operand(u);
+            for (int j = 0; j < kRT; j++) {
+              const int chunk = kDepth / 8 * t + part;
+              pb[t][j] = *reinterpret_cast<const bf16x8*>(sh.p[n & 1][kSize * j + pr] + 16 * (chunk ^ (pr >> 1 & 3)));
+            }
 #pragma unroll
-        for (int u = 0; u < kPvSteps; u++) {
-          const int i = u % kLT, t = u / kLT;
-          if (u + kRead < kPvSteps) v[u + kRead] = operand(u + kRead);
-          if (i < kRT && t + 1 < kGroups) pb[t + 1][i] = weights_of(t + 1, i);
-#pragma unroll
-          for (int j = 0; j < kRT; j++) {
-            if constexpr (kBig)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
-            else
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
-          }
-          if (u < kLoads - kInQk - kInSm) bring(b + 1, kInQk + kInSm + u);
-          if (kInt8 && u < kOwn) put_row(b + 1, u);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int u = 0; u < kRead; u++) v[u] = operand(u);
         }
-        static_assert(kOwn <= kPvSteps && kLoads - kInQk - kInSm <= kPvSteps, "every row has its step");
-      }
-    }
-    loads_done();   // what was asked for past the last block
-
-    // ---- the rows' sums and references, then the output or the partial
-    wg_barrier();
-    const int part = lane / kRowSize, c = lane & (kRowSize - 1);
-    if (takes_rows) {
-      const float l = kBig ? half_sum(sum) : quad_sum(sum);
-      const int row = kRowSize * rh + c;
-      if (lane < kRowSize) sh.red[kg][row] = l;
-      if (kg == 0 && lane < kRowSize) sh.ref[row] = ref;
-    }
-    wg_barrier();
-    auto sum_of = [&](int row) {
-      float l = sh.red[0][row] + sh.red[1][row];
-      if (!kBig) l += sh.red[2][row] + sh.red[3][row];
-      return l;
-    };
-    LateArgs* e = late_args();
-    if (!kSplit || (lo <= start && start + units <= hi)) {
-      // whole rows go out: as bf16 through LDS (chunk c of row r at c ^ (r %
-      // 8), so that rows fall on different banks), then each wave stores every
-      // kWaves-th row
-      uint8_t* os = sh.kv[0].lat[0];
+        auto between = [&](int u) {   // kPvSteps = 8: the loads and the conversion, in eighths
+          if constexpr (kInt8) {
+            convert(after, u, masks);
+            if (u < kLoads - 1) bring(into, u);
+          } else {
+            bring(into, u);
+            if (u == 7) bring(into, 8);
+          }
+          if (u == 7) look_up(n + kAhead + 2);
+        };
+        static_assert(kPvSteps == 8 && kOwn == 8, "a row a step");
+        auto steps = [&](int from, int to) {
+          if (n >= 0) {
 #pragma unroll
-      for (int j = 0; j < kRT; j++) {
-        const float l = sum_of(kRowSize * j + c);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+            for (int u = 0; u < kPvSteps; u++)
+              if (u >= from && u < to) {
+                const int i = u % kLT, t = u / kLT;
+                if (u + kRead < kPvSteps) v[u + kRead] = operand(u + kRead);
+#pragma unroll
+                for (int j = 0; j < kRT; j++) {
+                  if constexpr (kBig)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
+                  else
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
+                }
+                between(u);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+          } else {
+#pragma unroll
+            for (int u = 0; u < kPvSteps; u++)
+              if (u >= from && u < to) between(u);
+          }
+        };
+        steps(0, kFirst);
+        wg_barrier();   // the maxima
+        if (w == kHalf && lane == 0) sh.flag[n & 1] = 0;   // (block n + 2 sets it after this iteration)
+        steps(kFirst, kPvSteps);
+        loads_left<kLoads>();   // all but this iteration's: block n + 2's rows (INT8: n + 3's) are there
+        if (!kInt8 && (masks & 0xff) != 0xff) zero_rows(after, masks);
+        masks = kInt8 ? masks >> 8 | mask << 8 : mask;   // from block n + 3 on
+        wg_barrier();   // P
+        buf = next;
+      }
+      loads_left<0>();   // what was asked for past the last block
+      wg_barrier();
+      wg_barrier();      // the sums
+
+      // ---- the output as bf16 into LDS, or the partial
+      auto sum_of = [&](int row) { return sh.red[0][row] + sh.red[1][row]; };
+      const int part = lane / kSize, pr = lane & (kSize - 1);
+      if (!kSplit || (lo <= start && start + units <= hi)) {
+        // chunk c of 16 bytes of row r at c ^ (r % 8), so that rows fall on different banks
+        uint8_t* os = sh.kv[0].lat[0];
+#pragma unroll
+        for (int j = 0; j < kRT; j++) {
+          const float l = sum_of(kSize * j + pr);
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+          for (int i = 0; i < kLT; i++)
+#pragma unroll
+            for (int q = 0; q < kAcc; q += 4) {
+              const Acc v = acc[i][j];
+              const int lat = 128 * y + kSize * i + 2 * q + 4 * part;   // of v[q]
+              *reinterpret_cast<uint2*>(os + (kSize * j + pr) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (pr & 7))) + (2 * lat & 15)) =
+                  make_uint2(pack_bf16x2(v[q] * inv, v[q + 1] * inv), pack_bf16x2(v[q + 2] * inv, v[q + 3] * inv));
+            }
+        }
+      } else {
+        // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins
+        // here.  In the accumulators' order: 16 bytes of each lane at a time.
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (lo <= start);
+        float* out = e->part + static_cast<int64_t>(slot) * (kTM * kLatent);
 #pragma unroll
         for (int i = 0; i < kLT; i++)
 #pragma unroll
-          for (int q = 0; q < kAcc; q += 4) {
-            const Acc v = acc[i][j];
-            const int lat = kRowSize * (kLT * w + i) + (kBig ? 8 * (q / 4) : 0) + 4 * part;   // of v[q]
-            *reinterpret_cast<uint2*>(os + (kRowSize * j + c) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (c & 7))) + (2 * lat & 15)) =
-                make_uint2(pack_bf16x2(v[q] * inv, v[q + 1] * inv), pack_bf16x2(v[q + 2] * inv, v[q + 3] * inv));
-          }
+          for (int j = 0; j < kRT; j++)
+#pragma unroll
+            for (int q = 0; q < kAcc; q += 4) {
+              const Acc v = acc[i][j];
+              *reinterpret_cast<f32x4*>(out + (((kLT * y + i) * kRT + j) * (kAcc / 4) + q / 4) * 256 + 4 * lane) =
+                  f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+            }
+        if (y == 0 && lane < kTM)
+          e->ml[static_cast<int64_t>(slot) * kTM + lane] = make_float2(sh.alpha[0][lane], sum_of(lane));
+        if (lo <= start && y == 0 && lane == 0) {
+          const int64_t groups = min(static_cast<int>(gridDim.x), total);
+          // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
+          const int64_t last_unit = start + units;
+          e->shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
+        }
       }
+    }
+
+    if (!kSplit || (lo <= start && start + units <= hi)) {   // whole rows go out, every eighth of each wave's
       wg_barrier();
+      const uint8_t* os = sh.kv[0].lat[0];
       const int heads = e->heads, aligned = e->out_align16;
       const int64_t so_t = e->so_t, so_h = e->so_h;
       uint16_t* out = e->out;
@@ -787,37 +872,12 @@ __global__ __launch_bounds__(ChunkShape<kTM>::kThreads, 1) void chunk_mla_kernel
           reinterpret_cast<uint2*>(o)[2 * lane + 1] = make_uint2(v.z, v.w);
         }
         if (lse && lane == 0) {
-          const float l = sum_of(j);
+          const float l = sh.red[0][j] + sh.red[1][j];
           lse[static_cast<int64_t>(rq.t0 + tok) * heads + head] =
-              l == 0.f ? -INFINITY : (sh.ref[j] + __builtin_amdgcn_logf(l)) * kLn2;
+              l == 0.f ? -INFINITY : (sh.alpha[0][j] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
       if (kSplit && threadIdx.x == 0) e->shares[tile] = make_int2(-1, -1);
-    } else {
-      // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins
-      // here.  In the accumulators' order: 16 bytes of each lane at a time.
-      const int slot = 2 * static_cast<int>(blockIdx.x) + (lo <= start);
-      float* out = e->part + static_cast<int64_t>(slot) * (kTM * kLatent);
-#pragma unroll
-      for (int i = 0; i < kLT; i++)
-#pragma unroll
-        for (int j = 0; j < kRT; j++)
-#pragma unroll
-          for (int q = 0; q < kAcc; q += 4) {
-            const Acc v = acc[i][j];
-            *reinterpret_cast<f32x4*>(out + (((kLT * w + i) * kRT + j) * (kAcc / 4) + q / 4) * 256 + 4 * lane) =
-                f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
-          }
-      if (threadIdx.x < kTM) {
-        const int row = threadIdx.x;
-        e->ml[static_cast<int64_t>(slot) * kTM + row] = make_float2(sh.ref[row], sum_of(row));
-      }
-      if (lo <= start && threadIdx.x == 0) {
-        const int64_t groups = min(static_cast<int>(gridDim.x), total);
-        // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
-        const int64_t last_unit = start + units;
-        e->shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
-      }
     }
     if (!kSplit) return;
   }
@@ -941,14 +1001,14 @@ Workspace workspace_of(int tm, int64_t tiles) {
 template <int kTM, bool kInt8>
 int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
   if (a.num_tiles > kMaxSplitTiles) {
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(ChunkShape<kTM>::kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(kThreads), 0, st, a);
     // a shared tile has about CUs / tiles partials: 16 waves on a job where
     // that is many, one where it is few
     if (a.num_tiles <= 16)
@@ -1012,9 +1072,17 @@ extern "C" int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h, const 
   a.block_size = static_cast<int>(block_size);
   while (a.first_step < num_reqs && (a.first_step ? 2 * a.first_step : 1) < num_reqs)
     a.first_step = a.first_step ? 2 * a.first_step : 1;
+  int log2_block = 0;   // rounded up
+  while ((INT64_C(1) << log2_block) < block_size) log2_block++;
+  a.div_mul = static_cast<uint32_t>(((uint64_t(1) << log2_block) - static_cast<uint64_t>(block_size)) *
+                                        (uint64_t(1) << 32) / static_cast<uint64_t>(block_size) + 1);
+  a.div_sh1 = log2_block < 1 ? log2_block : 1, a.div_sh2 = log2_block > 1 ? log2_block - 1 : 0;
   a.num_reqs = static_cast<int>(num_reqs), a.total_q = static_cast<int>(total_q), a.heads = static_cast<int>(num_heads);
   a.num_tiles = static_cast<int>(tiles);
   a.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
+  // a scale of 0: the least that still leaves a masked logit -inf
+  if (a.scale_log2 == 0.f) a.scale_log2 = 1.17549435e-38f;
+  a.masked = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
   a.out = static_cast<uint16_t*>(out);
   a.so_t = so_t, a.so_h = so_h;
   a.out_align16 = oa % 16 == 0 && so_t % 8 == 0 && so_h % 8 == 0;

@@ -62,7 +62,13 @@ def _aligned16(t):
     """Whether t's rows can be read 16 bytes at a time: contiguous, every
     other stride and the base a multiple of 16 bytes."""
     size = t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in t.stride()[:-1])
+    *steps, last = t.stride()
+    if last != 1 or t.data_ptr() % 16:
+        return False
+    for s in steps:
+        if s * size % 16:
+            return False
+    return True
 
 
 def _rows16(t):
@@ -121,8 +127,9 @@ def store_rope(x, k_pe, positions, cos_sin, cache, slots, *, q_pe=None, q_out=No
     if q_pe is None and q_out is not None:
         raise ValueError("q_out without q_pe")
     dev = x.device
-    if not x.is_cuda or any(t is not None and t.device != dev
-                            for t in (k_pe, positions, cos_sin, cache, slots, q_pe, q_out, norm_weight)):
+    if not x.is_cuda or k_pe.device != dev or positions.device != dev or cos_sin.device != dev \
+            or cache.device != dev or slots.device != dev or (q_pe is not None and q_pe.device != dev) \
+            or (q_out is not None and q_out.device != dev) or (norm_weight is not None and norm_weight.device != dev):
         raise ValueError("store_rope requires CUDA (HIP) tensors on one device")
     heads = 0
     if q_pe is not None:
@@ -142,17 +149,18 @@ def store_rope(x, k_pe, positions, cos_sin, cache, slots, *, q_pe=None, q_out=No
     if norm_weight is not None:
         norm_weight = _rows16(norm_weight)
     positions, slots = positions.contiguous(), slots.contiguous()
-    page, block = cache.stride(0) * 2, cache.shape[1]
+    pages, block, _ = cache.shape
+    sq_t, sq_h = q_pe.stride()[:2] if heads else (0, 0)
+    so_t, so_h = q_out.stride()[:2] if heads else (0, 0)
     L = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = L.glm53_store_rope(
             x.data_ptr(), x.stride(0), k_pe.data_ptr(), k_pe.stride(0), positions.data_ptr(),
-            int(positions.dtype == torch.int64), cos_sin.data_ptr(), int(cos_sin.dtype == torch.float32),
-            cos_sin.shape[0], int(bool(interleaved)), norm_weight.data_ptr() if norm_weight is not None else None,
-            float(eps), cache.data_ptr(), page, cache.stride(1) * 2, max(block, 1), cache.shape[0] * block,
-            slots.data_ptr(), int(slots.dtype == torch.int64), n,
-            q_pe.data_ptr() if heads else None, q_pe.stride(0) if heads else 0, q_pe.stride(1) if heads else 0,
-            q_out.data_ptr() if heads else None, q_out.stride(0) if heads else 0, q_out.stride(1) if heads else 0,
-            heads, _lib.stream_handle(dev))
-    _lib.check(rc, "glm53_store_rope")
+            positions.dtype == torch.int64, cos_sin.data_ptr(), cos_sin.dtype == torch.float32, cos_sin.shape[0],
+            bool(interleaved), norm_weight.data_ptr() if norm_weight is not None else None, eps, cache.data_ptr(),
+            2 * cache.stride(0), 2 * cache.stride(1), max(block, 1), pages * block, slots.data_ptr(),
+            slots.dtype == torch.int64, n, q_pe.data_ptr() if heads else None, sq_t, sq_h,
+            q_out.data_ptr() if heads else None, so_t, so_h, heads, _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "glm53_store_rope")
     return q_out

@@ -415,15 +415,17 @@ def mla_chunk_attention_paged(
     if cu_seqlens_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.dtype != torch.int32:
         raise ValueError("cu_seqlens_q, seq_lens and block_table must be int32")
     R = seq_lens.numel()
-    if cu_seqlens_q.numel() != R + 1 or block_table.dim() != 2 or block_table.shape[0] != R:
+    if seq_lens.dim() != 1 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != R + 1 or block_table.dim() != 2 \
+            or block_table.shape[0] != R:
         raise ValueError(f"cu_seqlens_q must be [{R + 1}] and block_table [{R}, max_blocks] for seq_lens [{R}]")
     dev = q.device
-    if not q.is_cuda or any(t.device != dev for t in (kv_cache, cu_seqlens_q, seq_lens, block_table)):
+    if not q.is_cuda or kv_cache.device != dev or cu_seqlens_q.device != dev or seq_lens.device != dev \
+            or block_table.device != dev:
         raise ValueError("mla_chunk_attention_paged requires CUDA (HIP) tensors on one device")
-    size = kv_cache.element_size()
-    page_bytes, row_bytes = kv_cache.stride(0) * size, kv_cache.stride(1) * size
-    if kv_cache.stride(2) != 1 or page_bytes % 16 or row_bytes % 16 or row_bytes < width * size \
-            or kv_cache.data_ptr() % 16:
+    size = 1 if int8 else 2
+    page_step, row_step, step = kv_cache.stride()
+    page_bytes, row_bytes, kv_ptr = page_step * size, row_step * size, kv_cache.data_ptr()
+    if step != 1 or page_bytes % 16 or row_bytes % 16 or row_bytes < width * size or kv_ptr % 16:
         raise ValueError("cache rows must be contiguous, 16-byte aligned, their strides multiples of 16 bytes")
     if out is None:
         out = torch.empty((T, H, _BLOCK_DV), dtype=torch.bfloat16, device=dev)
@@ -433,25 +435,36 @@ def mla_chunk_attention_paged(
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T == 0 or R == 0:
         return (out, lse) if return_lse else out
-    if q.stride(2) != 1 or q.stride(1) % 8 or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
+    sq_t, sq_h, step = q.stride()
+    if step != 1 or sq_h % 8 or sq_t % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        sq_t, sq_h, _ = q.stride()
     if block_table.stride(1) != 1:
         block_table = block_table.contiguous()
-    cu_seqlens_q, seq_lens = cu_seqlens_q.contiguous(), seq_lens.contiguous()
+    if cu_seqlens_q.stride(0) != 1:
+        cu_seqlens_q = cu_seqlens_q.contiguous()
+    if seq_lens.stride(0) != 1:
+        seq_lens = seq_lens.contiguous()
 
     L = _lib.load()
-    with torch.cuda.device(dev):
-        ws_bytes = L.glm53_chunk_mla_workspace_bytes(T, R, H)
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+    with _lib.on_device(dev):
+        ws_bytes = _chunk_workspace_bytes(T, R, H, dev.index)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = L.glm53_chunk_mla(
-            q.data_ptr(), q.stride(0), q.stride(1), kv_cache.data_ptr(), int(int8), page_bytes, row_bytes,
-            kv_cache.shape[0], kv_cache.shape[1], cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
-            block_table.data_ptr(), R, block_table.stride(0), block_table.shape[1], T, H, float(sm_scale),
-            workspace.data_ptr() if workspace is not None else None, ws_bytes,
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if lse is not None else None,
-            _lib.stream_handle(dev))
-    _lib.check(rc, "glm53_chunk_mla")
+            q.data_ptr(), sq_t, sq_h, kv_ptr, int8, page_bytes, row_bytes, kv_cache.shape[0], kv_cache.shape[1],
+            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), R, block_table.stride(0),
+            block_table.shape[1], T, H, sm_scale, workspace.data_ptr() if ws_bytes else None, ws_bytes,
+            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None,
+            _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "glm53_chunk_mla")
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _chunk_workspace_bytes(total_q, num_reqs, num_heads, device_index):
+    """glm53_chunk_mla_workspace_bytes on the current device."""
+    return int(_lib.load().glm53_chunk_mla_workspace_bytes(total_q, num_reqs, num_heads))
 
 
 def sparse_mla_partials(q, kv, indices, sm_scale, num_kv_splits):

@@ -11,6 +11,8 @@ host synchronisation, so the call is graph-capturable.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 import _glm53_lib as _lib
@@ -70,29 +72,34 @@ def verify_drafts(target_probs: torch.Tensor, draft_ids: torch.Tensor, draft_pro
     if R > _MAX_REQUESTS_PER_CALL:
         raise ValueError(f"at most {_MAX_REQUESTS_PER_CALL} requests per call, got {R}")
     dev = target_probs.device
-    if not target_probs.is_cuda or any(t is not None and t.device != dev
-                                       for t in (draft_ids, draft_probs, cu_rows, accept_u, sample_u)):
+    if not target_probs.is_cuda or draft_ids.device != dev or cu_rows.device != dev or accept_u.device != dev \
+            or sample_u.device != dev or (draft_probs is not None and draft_probs.device != dev):
         raise ValueError("verify_drafts requires CUDA (HIP) tensors on one device")
     tokens = torch.empty((R, max_drafts + 1), dtype=torch.int32, device=dev)
-    accepted = torch.empty((R,), dtype=torch.int32, device=dev)
+    accepted = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0:
         return tokens, accepted
     if target_probs.stride(1) != 1:
         target_probs = target_probs.contiguous()
-    if draft_probs is not None and draft_probs.stride(1) != 1:
+    with_probs = draft_probs is not None and D > 0
+    if with_probs and draft_probs.stride(1) != 1:
         draft_probs = draft_probs.contiguous()
     draft_ids, cu_rows = draft_ids.contiguous(), cu_rows.contiguous()
     accept_u, sample_u = accept_u.contiguous(), sample_u.contiguous()
     L = _lib.load()
-    with torch.cuda.device(dev):
-        ws_bytes = L.glm53_verify_drafts_workspace_bytes(R, vocab)
+    with _lib.on_device(dev):
+        ws_bytes = _workspace_bytes(R, vocab)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         rc = L.glm53_verify_drafts(
-            target_probs.data_ptr(), target_probs.stride(0), rows,
-            draft_probs.data_ptr() if draft_probs is not None and D else None,
-            draft_probs.stride(0) if draft_probs is not None else 0, draft_ids.data_ptr(),
-            int(draft_ids.dtype == torch.int64), D, cu_rows.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
-            R, vocab, max_drafts, workspace.data_ptr(), ws_bytes, tokens.data_ptr(), accepted.data_ptr(),
-            _lib.stream_handle(dev))
-    _lib.check(rc, "glm53_verify_drafts")
+            target_probs.data_ptr(), target_probs.stride(0), rows, draft_probs.data_ptr() if with_probs else None,
+            draft_probs.stride(0) if with_probs else 0, draft_ids.data_ptr(), draft_ids.dtype == torch.int64, D,
+            cu_rows.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), R, vocab, max_drafts, workspace.data_ptr(),
+            ws_bytes, tokens.data_ptr(), accepted.data_ptr(), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, "glm53_verify_drafts")
     return tokens, accepted
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(requests, vocab):
+    return int(_lib.load().glm53_verify_drafts_workspace_bytes(requests, vocab))
