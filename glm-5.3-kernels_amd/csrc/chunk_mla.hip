@@ -21,14 +21,15 @@
 //     each with the output in registers, and the loads.  bf16 rows come into a
 //     ring of four blocks in LDS by direct global -> LDS loads, three blocks
 //     ahead; INT8 rows as they are, four ahead, converted to bf16 once, two
-//     blocks before their use as V.  The block table's entries come the same
-//     way, two blocks before the loads that need them: nothing waits for memory
-//     but the count of outstanding loads, once a block.
-// The softmax goes against a reference maximum that moves only when a row's
-// maximum passes it by 2^8, so that the output is seldom rescaled; sums, output
-// and references are fp32.  P goes through LDS as bf16; V is read from the rows
-// that served as K, with transposing reads.  Two barriers a block: after the
-// row maxima (halves of the keys are in two waves) and after P.
+//     blocks before their use as V.  Nothing waits for memory but the count of
+//     outstanding loads, once a block: the block table's entries come ahead too.
+// The softmax goes against a row's reference, which stays until a logit passes
+// it by 2^16 (in the first block, and seldom after it): then the block is
+// weighted again with the row's maximum for a reference, and the output is
+// rescaled.  So a block costs one barrier, and the two waves that share a row
+// exchange their maxima only then.  Sums, output and references are fp32.  P
+// goes through LDS as bf16; V is read from the rows that served as K, with
+// transposing reads.
 // Few tiles (decode): the blocks of all tiles are laid end to end and cut
 // into equal runs, one per workgroup; a tile that several workgroups share
 // leaves fp32 partials that the merge kernel joins.  Many tiles: one
@@ -47,7 +48,7 @@ constexpr int kRope = 64;
 constexpr int kKeys = 32;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.f;       // how far (log2) a row's maximum may pass the reference
+constexpr float kSlack = 16.f;      // how far (log2) a logit may pass its row's reference
 
 struct ChunkArgs {
   const uint16_t* q;
@@ -69,7 +70,7 @@ struct ChunkArgs {
   int heads;
   int num_tiles;   // bound: tile indexes are below it
   float scale_log2;
-  float masked;    // -inf over the scale's sign: a masked logit before its scale
+  uint32_t flip;   // a negative scale: the sign bits of two bf16, for the queries
   uint16_t* out;
   int64_t so_t, so_h;
   int out_align16; // out rows 16-byte aligned (else 8)
@@ -107,14 +108,14 @@ struct __attribute__((aligned(16))) ChunkShared {
   float raw_scale[kInt8 ? 3 : 0][kKeys];
   float scl[kInt8 ? 3 : 0][kKeys];              // the scales, 0 for a key without a row
   uint8_t p[2][kTM][2 * kKeys];        // P, chunk c of 16 bytes of row r at c ^ (r / 2 % 4)
-  int32_t page[8][kKeys];              // block table entries of the coming blocks
+  int32_t page[kHalf * 64];            // block table entries of the coming blocks
   float red[2][kTM];                   // per key half: maxima; at the end the sums
-  float alpha[2][kTM];                 // what a block's new references scale the output with; at the end the references
+  float alpha[kTM];                    // what new references scale the output with; at the end the references
   int ends[kMaxSplitTiles];            // blocks up to and with each tile
   int reqs[kMaxSplitTiles];
-  uint8_t have[4][kHalf];              // bit j of byte y: key 8 y + j of the block has a row
-  int flag[2];                         // some reference moved
-  int sums[kWaves];
+  uint8_t have[8][kHalf];              // bit j of byte y: key 8 y + j of the block has a row
+  int again[2];                        // the last (odd, even) block that is weighted again
+  int sums[kWaves], tiles[kWaves];
   int first, first_t0, first_n, first_len;   // the first tile and its request
 };
 
@@ -129,21 +130,33 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)(p)));
 }
 
-// 16 bytes per lane from base + off to LDS at dst + 16 * lane.  Written in asm
-// so that the compiler does not wait for it before other LDS reads;
-// loads_left() and a barrier come before the first read of what it brings.
-// (m0 needs a wait state before its use, an SGPR from v_readlane five.  The
-// compiler keeps m0 out of clobber lists and sets it before each use of its
-// own; nothing else here uses it.)
+// 16 bytes per lane from base + off to LDS at dst + 16 * lane, and the same
+// for off2, ... at dst + 1024 + 16 * lane, ...  Written in asm so that the
+// compiler does not wait for it before other LDS reads; loads_left() and a
+// barrier come before the first read of what it brings.  (m0 needs a wait
+// state before its use, an SGPR from v_readlane five.  The compiler keeps m0
+// out of clobber lists and sets it before each use of its own; nothing else
+// here uses it.)
 __device__ __forceinline__ void load_lds16(uint32_t dst, const uint8_t* base, uint32_t off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base)
                : "memory");
+}
+__device__ __forceinline__ void load_lds16_2(uint32_t dst, const uint8_t* base, uint32_t off, uint32_t off2) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(dst),
+      "v"(off), "v"(off2), "s"(base)
+      : "memory", "scc");
 }
 __device__ __forceinline__ void load_lds16_at(uint32_t dst, const uint8_t* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(p) : "memory");
 }
 
-__device__ __forceinline__ void load_lds4_at(uint32_t dst, const void* p) {   // 4 bytes per lane
+// 4 bytes per lane to LDS at dst + 4 * lane
+__device__ __forceinline__ void load_lds4(uint32_t dst, const void* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds4_at(uint32_t dst, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(p) : "memory");
 }
 
@@ -242,7 +255,9 @@ __device__ __forceinline__ int divide(uint32_t n, uint32_t mul, int sh1, int sh2
   return static_cast<int>((t + ((n - t) >> sh1)) >> sh2);
 }
 
-template <int kTM, bool kInt8, bool kSplit>
+// kRuns: pages of a multiple of eight rows, so that the eight rows of a block
+// that a wave brings in lie behind one another in one page.
+template <int kTM, bool kInt8, bool kSplit, bool kRuns>
 __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
   using Shared = ChunkShared<kTM, kInt8>;
   constexpr bool kBig = ChunkShape<kTM>::kBig;
@@ -255,7 +270,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   constexpr int kBufs = Shared::kBufs;
   constexpr int kAhead = kInt8 ? 4 : 3;            // blocks between a row's load and its use as V
   constexpr int kEarly = kAhead - 1;               // blocks that are asked for before the loop
-  constexpr int kLoads = kInt8 ? 6 : 10;           // loads a latent wave sends per block
+  constexpr int kRowLoads = kInt8 ? 5 : 9;         // loads a latent wave sends per block for rows,
+  constexpr int kLoads = kRowLoads + !kRuns;       // and with those for table entries
   using Acc = std::conditional_t<kBig, f32x16, f32x4>;
   constexpr int kAcc = kBig ? 16 : 4;
   __shared__ Shared sh;
@@ -266,7 +282,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
   // ---- which blocks of which tiles are this workgroup's
-  int tile, lo = 0, hi = 0, total = 0;
+  int tile, lo = 0, hi = 0, total = 0, groups = 1;
   if (kSplit) {
     constexpr int kTiles = kMaxSplitTiles / kThreads;   // tiles of a thread
     int units[kTiles], req[kTiles], sum = 0;
@@ -299,23 +315,31 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       const int v = __shfl_up(upto, d);
       if (lane >= d) upto += v;
     }
-    if (lane == 63) sh.sums[w] = upto;
+    int filled = 0;
+#pragma unroll
+    for (int k = 0; k < kTiles; k++) filled += __popcll(__ballot(units[k] > 0));
+    if (lane == 63) sh.sums[w] = upto, sh.tiles[w] = filled;
     if (threadIdx.x == 0) sh.first = 0;
     wg_barrier();
-    int before = 0;
+    int before = 0, tiles = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; i++) {
       const int s = sh.sums[i];
       if (i < w) before += s;
       total += s;
+      tiles += sh.tiles[i];
     }
-    total = uniform(total);
+    total = uniform(total), tiles = uniform(tiles);
     if (total == 0) {
       if (blockIdx.x == 0)
         for (int t = threadIdx.x; t < a.num_tiles; t += kThreads) a.shares[t] = make_int2(-1, -1);
       return;   // uniform over the workgroup
     }
-    const int64_t groups = min(static_cast<int>(gridDim.x), total);
+    // A run of u blocks takes u times a block's time, and its partial (written,
+    // read, joined) kTM / 512 of that: the sum of both is least with
+    // sqrt(total * 512 / kTM) runs.  No fewer than tiles: those come without partials.
+    const int best = max(tiles, static_cast<int>(sqrtf(static_cast<float>(total) * (512 / kTM))));
+    groups = min(min(static_cast<int>(gridDim.x), total), best);
     if (static_cast<int>(blockIdx.x) >= groups) return;
     lo = static_cast<int>(blockIdx.x * static_cast<int64_t>(total) / groups);
     hi = static_cast<int>((blockIdx.x + 1) * static_cast<int64_t>(total) / groups);
@@ -428,34 +452,91 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           if constexpr (!kInt8) {
             if (st >= 16) from = qs.rope[key & 31] + 16 * ((4 * (st - 16) + g) ^ sw);
           }
-          qf[rt][st] = *reinterpret_cast<const bf16x8*>(from);
+          const uint4 v = *reinterpret_cast<const uint4*>(from);
+          qf[rt][st] = __builtin_bit_cast(bf16x8, make_uint4(v.x ^ a.flip, v.y ^ a.flip, v.z ^ a.flip, v.w ^ a.flip));
         }
       }
       wg_barrier();   // the queries have been read
-      // the reference maxima (log2) of this lane's rows, from the least number on: every other logit passes it
+      // the references (log2) of this lane's rows, from the least number on: every logit passes it
       float ref[kRQ], sum[kRQ];
 #pragma unroll
       for (int rt = 0; rt < kRQ; rt++) ref[rt] = -3.4028234663852886e38f, sum[rt] = 0.f;
+      f32x4 s[kRQ] = {};            // the last block's logits (log2)
+      float part_sum[kRQ] = {};     // its part of the sums
+      float ksv[4] = {1.f, 1.f, 1.f, 1.f};
+      // The weights of block n, for PV.
+      auto weigh = [&](int n) {
+#pragma unroll
+        for (int rt = 0; rt < kRQ; rt++) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(s[rt][i] - ref[rt]);
+          part_sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+          if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] *= ksv[i];
+          }
+          // P is rounded to bf16 (like the output, 2^-9 of each weight on
+          // the average); the sum keeps the unrounded weights.  With the
+          // small products of PV the operand's keys are 4 g + i, 16 + 4 g + i.
+          const int chunk = kBig ? 2 * kh + (g >> 1) : g, half = kBig ? g & 1 : kh;
+          *reinterpret_cast<uint2*>(sh.p[n & 1][16 * (rh * kRQ + rt) + c] + 16 * (chunk ^ (c >> 1 & 3)) + 8 * half) =
+              make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
+        }
+      };
       int buf = 0;
-      for (int n = 0; n < count; n++) {
+      for (int n = 0;; n++) {
         // ---- S^T = K Q^T: keys 16 kh + 4 g + i of block n, rows c.  Each
         // K-step's operand is read some steps before its products.
-        f32x4 s[kRQ];
-        float ksv[4] = {1.f, 1.f, 1.f, 1.f};
-        if (takes_rows) {
-          constexpr int kRead = 6;
-          const int key = 16 * kh + c, sw = swizzle(c);
-          const auto& blk = sh.kv[buf];
-          const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
-          const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
-          auto operand = [&](int st) {
-            const uint8_t* from = (st & 1 ? odd : even) + 128 * (st >> 1);
-            if constexpr (!kInt8) {
-              if (st >= 16) from = blk.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
+        constexpr int kRead = 6;
+        const int key = 16 * kh + c, sw = swizzle(c);
+        const auto& blk = sh.kv[buf];
+        const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
+        const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
+        auto operand = [&](int st) {
+          const uint8_t* from = (st & 1 ? odd : even) + 128 * (st >> 1);
+          if constexpr (!kInt8) {
+            if (st >= 16) from = blk.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
+          }
+          return *reinterpret_cast<const bf16x8*>(from);
+        };
+        bf16x8 k[kSteps];
+        const int again = sh.again[(n & 1) ^ 1];
+        const uint32_t have_v = static_cast<uint32_t>(*reinterpret_cast<const int*>(sh.have[n & 7]));
+        if (takes_rows) {   // (after the last block: not used)
+#pragma unroll
+          for (int st = 0; st < kRead; st++) k[st] = operand(st);
+        }
+        if (n && uniform(again) == n - 1) {
+          // ---- the block before again: both waves of a row find its reference
+          float top[kRQ];
+          if (takes_rows) {
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++) {
+              top[rt] = quad_max(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3])));
+              if (lane < 16) sh.red[kh][16 * (rh * kRQ + rt) + c] = top[rt];
             }
-            return *reinterpret_cast<const bf16x8*>(from);
-          };
-          const uint32_t have = static_cast<uint32_t>(*reinterpret_cast<const int*>(sh.have[n & 3]));
+          }
+          wg_barrier();   // the maxima
+          if (takes_rows) {
+#pragma unroll
+            for (int rt = 0; rt < kRQ; rt++) {
+              const int row = 16 * (rh * kRQ + rt) + c;
+              const float m = fmaxf(ref[rt], fmaxf(sh.red[0][row], sh.red[1][row]));
+              const float alpha = __builtin_amdgcn_exp2f(ref[rt] - m);
+              ref[rt] = m;
+              sum[rt] *= alpha;
+              if (kh == 0 && lane < 16) sh.alpha[row] = alpha;
+            }
+            weigh(n - 1);
+          }
+          wg_barrier();   // P
+        }
+#pragma unroll
+        for (int rt = 0; rt < kRQ; rt++) sum[rt] += part_sum[rt];
+        if (n == count) break;
+        if (takes_rows) {
+          const uint32_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v)));
           if constexpr (kInt8) {
             const float4 v = *reinterpret_cast<const float4*>(&sh.scl[buf][16 * kh + 4 * g]);
             ksv[0] = v.x, ksv[1] = v.y, ksv[2] = v.z, ksv[3] = v.w;
@@ -467,9 +548,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           for (int rt = 0; rt < kRQ; rt++)
 #pragma unroll
             for (int u = 0; u < kSums; u++) t[rt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-          bf16x8 k[kSteps];
-#pragma unroll
-          for (int st = 0; st < kRead; st++) k[st] = operand(st);
 #pragma unroll
           for (int st = 0; st < kSteps; st++) {
             if (st + kRead < kSteps) k[st + kRead] = operand(st + kRead);
@@ -478,15 +556,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
               t[rt][st % kSums] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], t[rt][st % kSums], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
           }
+          float scale[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) scale[i] = kInt8 ? a.scale_log2 * ksv[i] : a.scale_log2;
 #pragma unroll
           for (int rt = 0; rt < kRQ; rt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              s[rt][i] = kSums == 1 ? t[rt][0][i] : t[rt][0][i] + t[rt][kSums - 1][i];
-              // bf16: the logits keep their scale until their weights are taken
-              if constexpr (kInt8) s[rt][i] *= a.scale_log2 * ksv[i];
-            }
-          if (uniform(static_cast<int>(have)) != -1 || (b0 + n + 1) * kKeys - 1 > least) {
+            for (int i = 0; i < 4; i++)
+              s[rt][i] = (kSums == 1 ? t[rt][0][i] : t[rt][0][i] + t[rt][kSums - 1][i]) * scale[i];
+          if (have != ~0u || (b0 + n + 1) * kKeys - 1 > least) {
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++) {
               const int row = min(row0 + 16 * (rh * kRQ + rt) + c, rows - 1);
@@ -495,7 +573,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
               for (int i = 0; i < 4; i++) {
                 const int key = 16 * kh + 4 * g + i;
-                if (key > limit || !(have >> key & 1)) s[rt][i] = kInt8 ? -INFINITY : a.masked;
+                if (key > limit || !(have >> key & 1)) s[rt][i] = -INFINITY;
               }
             }
           }
@@ -505,77 +583,24 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int i = 0; i < 4; i++) ksv[i] = fabsf(ksv[i]) < INFINITY ? ksv[i] : 0.f;
           }
+          bool far = false;
 #pragma unroll
-          for (int rt = 0; rt < kRQ; rt++) {
-            float top;
-            if (kInt8 || a.scale_log2 >= 0.f)
-              top = fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]));
-            else
-              top = fminf(fminf(s[rt][0], s[rt][1]), fminf(s[rt][2], s[rt][3]));
-            if constexpr (!kInt8) top *= a.scale_log2;
-            top = quad_max(top);
-            if (lane < 16) sh.red[kh][16 * (rh * kRQ + rt) + c] = top;
-          }
-        }
-        wg_barrier();   // the maxima
-        if (takes_rows) {
-          // ---- softmax: a row's reference moves where its maximum passed it
-          // by 2^8; both waves of a row decide alike
-          bool moved = false;
-          float scaled[kRQ];
-#pragma unroll
-          for (int rt = 0; rt < kRQ; rt++) {
-            const int row = 16 * (rh * kRQ + rt) + c;
-            const float m = fmaxf(sh.red[0][row], sh.red[1][row]);
-            scaled[rt] = ref[rt];
-            if (m > ref[rt] + kSlack) ref[rt] = m, moved = true;
-          }
-          if (__ballot(moved)) {
-#pragma unroll
-            for (int rt = 0; rt < kRQ; rt++) {
-              const float alpha = __builtin_amdgcn_exp2f(scaled[rt] - ref[rt]);
-              sum[rt] *= alpha;
-              if (kh == 0 && lane < 16) sh.alpha[n & 1][16 * (rh * kRQ + rt) + c] = alpha;
-            }
-            if (lane == 0) sh.flag[n & 1] = 1;
-          } else if (kh == 0 && lane < 16) {   // the other row half's may have moved
-#pragma unroll
-            for (int rt = 0; rt < kRQ; rt++) sh.alpha[n & 1][16 * (rh * kRQ + rt) + c] = 1.f;
-          }
-#pragma unroll
-          for (int rt = 0; rt < kRQ; rt++) {
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              p[i] = __builtin_amdgcn_exp2f(kInt8 ? s[rt][i] - ref[rt] : __builtin_fmaf(s[rt][i], a.scale_log2, -ref[rt]));
-            sum[rt] += (p[0] + p[1]) + (p[2] + p[3]);
-            if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
-#pragma unroll
-              for (int i = 0; i < 4; i++) p[i] *= ksv[i];
-            }
-            // P is rounded to bf16 (like the output, 2^-9 of each weight on
-            // the average); the sum keeps the unrounded weights.  With the
-            // small products of PV the operand's keys are 4 g + i, 16 + 4 g + i.
-            const int chunk = kBig ? 2 * kh + (g >> 1) : g, half = kBig ? g & 1 : kh;
-            *reinterpret_cast<uint2*>(sh.p[n & 1][16 * (rh * kRQ + rt) + c] + 16 * (chunk ^ (c >> 1 & 3)) + 8 * half) =
-                make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
-          }
+          for (int rt = 0; rt < kRQ; rt++)
+            far |= fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3])) > ref[rt] + kSlack;
+          if (far) sh.again[n & 1] = n;
+          weigh(n);
         }
         wg_barrier();   // P
         buf = buf + 1 < kBufs ? buf + 1 : 0;
       }
-      if (count) {   // PV of the last block
-        wg_barrier();
-        wg_barrier();
-      }
-      wg_barrier();   // PV has read P and the references' changes for the last time
+      if (count) wg_barrier();   // PV has read P and the rescaling for the last time
       if (takes_rows) {
 #pragma unroll
         for (int rt = 0; rt < kRQ; rt++) {
           const float l = quad_sum(sum[rt]);
           const int row = 16 * (rh * kRQ + rt) + c;
           if (lane < 16) sh.red[kh][row] = l;
-          if (kh == 0 && lane < 16) sh.alpha[0][row] = ref[rt];
+          if (kh == 0 && lane < 16) sh.alpha[row] = ref[rt];
         }
       }
       wg_barrier();   // the sums
@@ -583,57 +608,109 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       // ================ latents: loads, PV
       const int y = w - kHalf;
       // ---- bringing blocks in, counted from the first (block n has the
-      // positions 32 (b0 + n) + [0, 32)).  Wave y brings in rows 8 y .. 8 y + 7;
-      // lane l looks after row 8 y + l / 8: its page from the table, then its
-      // address.  A key past the last one seen, or whose page is not in the
-      // table or the cache, has no row: the cache's first is read in its place
-      // and zeroed, so that every wave sends kLoads loads a block, also for
-      // blocks past the end.
+      // positions 32 (b0 + n) + [0, 32)).  Wave y brings in rows 8 y .. 8 y + 7.
+      // A key past the last one seen, or whose page is not in the table or the
+      // cache, has no row: the cache's first is read in its place (or, past the
+      // last one, what the page has there), and zeroed if it is bf16, so that
+      // every wave sends kLoads loads a block, also for blocks past the end.
+      //
+      // With kRuns the wave needs one table entry a block: lane l keeps that of
+      // block l of 64, and the next 64 come while they are used.  Without, lane
+      // l looks after row l / 8 (INT8: l % 8).
       const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
-      auto look_up = [&](int n) {       // the block table's entries for block n, by every wave
-        const int pos = min((b0 + n) * kKeys + (lane & 31), last);
-        const int pg = divide(pos, a.div_mul, a.div_sh1, a.div_sh2);
-        if (lane < 32) load_lds4_at(lds_offset(sh.page[n & 7]), bt + pg);
+      auto look_up = [&](int n) {       // the table's entries for block n, kRuns: for blocks n .. n + 63
+        const int64_t at = kRuns ? (b0 + n + lane) * static_cast<int64_t>(kKeys) + kOwn * y : (b0 + n) * kKeys + (lane & 31);
+        const int pg = divide(static_cast<int>(at < last ? at : last), a.div_mul, a.div_sh1, a.div_sh2);
+        if constexpr (kRuns) {
+          load_lds4_at(lds_offset(&sh.page[64 * y]), bt + pg);
+        } else {
+          if (lane < 32) load_lds4_at(lds_offset(&sh.page[32 * (n & 7)]), bt + pg);   // by every wave
+        }
       };
-      uint32_t row_lo = 0, row_hi = 0, masks = 0;   // masks: a byte per block on its way, this wave's rows
+      uint32_t masks = 0;               // a byte per block on its way, of this wave's rows
+      int pages = 0;                    // kRuns
+      uint64_t run = 0;                 // kRuns: the address of the eight rows
+      uint32_t row_lo = 0, row_hi = 0;  // of the lane's row, without kRuns
+      uint32_t row_off[kRuns ? kRowLoads : 1];
+      if constexpr (kRuns) {
+        const uint32_t rb = static_cast<uint32_t>(a.row_bytes);
+#pragma unroll
+        for (int j = 0; j < kRowLoads; j++) {
+          if (kInt8)
+            row_off[j] = j < 4 ? (2 * j + (lane >> 5)) * rb + 16 * (lane & 31) : (lane & 7) * rb + kLatent;
+          else
+            row_off[j] = j < kOwn ? j * rb + ((16 * lane) ^ (16 * swizzle(j)))
+                                  : (lane >> 3) * rb + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3));
+        }
+      }
+      const int of_lane = kInt8 ? lane & 7 : lane >> 3;
+      // where block n's rows are; what of them there is, a bit each
       auto address = [&](int n) {
-        const int key = kOwn * y + (lane >> 3), pos = (b0 + n) * kKeys + key;
-        const int page = sh.page[n & 7][key];
-        const int in_page = pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size;
-        const bool ok = n < count && pos <= last && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
-        const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
-                            (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
-        row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
-        // bit 8 j of the ballot to bit j
-        const uint32_t mask = static_cast<uint32_t>(((__ballot(ok) & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
-        if (lane == 0) sh.have[n & 3][y] = static_cast<uint8_t>(mask);
+        uint32_t mask;
+        if constexpr (kRuns) {
+          if ((n & 63) == 0) pages = sh.page[64 * y + lane];
+          const uint32_t page = static_cast<uint32_t>(__builtin_amdgcn_readlane(pages, n & 63));
+          const int pos = (b0 + n) * kKeys + kOwn * y;
+          const uint32_t in_page = static_cast<uint32_t>(pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size);
+          const int left = n < count && page < static_cast<uint32_t>(a.num_blocks) ? last - pos + 1 : 0;
+          mask = left >= kOwn ? 0xffu : left > 0 ? (1u << left) - 1 : 0u;
+          run = reinterpret_cast<uint64_t>(a.kv) +
+                (mask ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
+        } else {
+          const int key = kOwn * y + of_lane, pos = (b0 + n) * kKeys + key;
+          const int page = sh.page[32 * (n & 7) + key];
+          const int in_page = pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size;
+          const bool ok = n < count && pos <= last && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
+          const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
+                              (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
+          row_lo = static_cast<uint32_t>(at), row_hi = static_cast<uint32_t>(at >> 32);
+          const uint64_t all = __ballot(ok);
+          // INT8: the low byte; bf16: bit 8 j to bit j
+          mask = kInt8 ? static_cast<uint32_t>(all) & 0xff
+                       : static_cast<uint32_t>(((all & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+        }
+        if (lane == 0) sh.have[n & 7][y] = static_cast<uint8_t>(mask);
         return mask;
       };
       auto row_of = [&](int j) {        // uniform: row j of the wave's
-        return reinterpret_cast<const uint8_t*>(
-            static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, 8 * j)) |
-            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, 8 * j))) << 32);
+        const int from = kInt8 ? j : 8 * j;
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(row_lo, from)) |
+               static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row_hi, from))) << 32;
       };
-      auto row_at = [&](int j) {        // per lane
-        return reinterpret_cast<const uint8_t*>(
-            static_cast<uint32_t>(__shfl(static_cast<int>(row_lo), 8 * j)) |
-            static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(row_hi), 8 * j))) << 32);
-      };
-      // load j of kLoads - 1 of block n's rows into buffer `to`
+      // loads 2 j and 2 j + 1 (of kRowLoads) of the block whose addresses are there into buffer `to`
+      constexpr int kPairs = (kRowLoads + 1) / 2;
       auto bring = [&](int to, int j) {
+        const uint8_t* own = reinterpret_cast<const uint8_t*>(row_lo | static_cast<uint64_t>(row_hi) << 32);
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(run);
         if constexpr (kInt8) {
-          if (j < 4)
-            load_lds16_at(lds_offset(sh.raw[to][kOwn * y + 2 * j]), row_at(2 * j + (lane >> 5)) + 16 * (lane & 31));
-          else {
-            const uint8_t* row = row_at(lane & 7);
-            if (lane < kOwn) load_lds4_at(lds_offset(&sh.raw_scale[to][kOwn * y]), row + kLatent);
+          const uint32_t dst = lds_offset(sh.raw[to][kOwn * y + 4 * j]);
+          if (j == 2) {
+            if (lane < kOwn) {
+              if constexpr (kRuns)
+                load_lds4(lds_offset(&sh.raw_scale[to][kOwn * y]), base, row_off[kRowLoads - 1]);
+              else
+                load_lds4_at(lds_offset(&sh.raw_scale[to][kOwn * y]), own + kLatent);
+            }
+          } else if constexpr (kRuns) {
+            load_lds16_2(dst, base, row_off[2 * j], row_off[2 * j + 1]);
+          } else {
+            for (int i = 0; i < 2; i++) {
+              const uint64_t row = lane < 32 ? row_of(4 * j + 2 * i) : row_of(4 * j + 2 * i + 1);
+              load_lds16_at(dst + 1024 * i, reinterpret_cast<const uint8_t*>(row) + 16 * (lane & 31));
+            }
           }
         } else {
-          if (j < kOwn) {
-            load_lds16(lds_offset(sh.kv[to].lat[kOwn * y + j]), row_of(j), (16 * lane) ^ (16 * swizzle(j)));
+          const uint32_t dst = lds_offset(sh.kv[to].lat[kOwn * y + 2 * j]);
+          if (j == 4) {
+            if constexpr (kRuns)
+              load_lds16(lds_offset(sh.kv[to].rope[kOwn * y]), base, row_off[kRowLoads - 1]);
+            else
+              load_lds16_at(lds_offset(sh.kv[to].rope[kOwn * y]), own + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3)));
+          } else if constexpr (kRuns) {
+            load_lds16_2(dst, base, row_off[2 * j], row_off[2 * j + 1]);
           } else {
-            const uint8_t* row = reinterpret_cast<const uint8_t*>(row_lo | static_cast<uint64_t>(row_hi) << 32);
-            load_lds16_at(lds_offset(sh.kv[to].rope[kOwn * y]), row + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3)));
+            for (int i = 0; i < 2; i++)
+              load_lds16(dst + 1024 * i, reinterpret_cast<const uint8_t*>(row_of(2 * j + i)), (16 * lane) ^ (16 * swizzle(2 * j + i)));
           }
         }
       };
@@ -646,41 +723,50 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             }
         }
       };
-      // INT8: row j of the wave's from raw block `in` to the bf16 block there (0 without a row)
-      auto convert = [&](int in, int j, uint32_t mask) {
+      // INT8: row j of the wave's in raw block `in`, and as bf16 into the block
+      // there (without a row: any codes, with the scale 0)
+      auto codes_of = [&](int in, int j) {
+        if constexpr (kInt8)
+          return *reinterpret_cast<const uint2*>(&sh.raw[in][kOwn * y + j][8 * lane]);
+        else
+          return make_uint2(0, 0);
+      };
+      auto convert = [&](int in, int j, uint2 v, uint32_t mask) {
         if constexpr (kInt8) {
-          const uint2 v = *reinterpret_cast<const uint2*>(&sh.raw[in][kOwn * y + j][8 * lane]);
-          const uint32_t keep = 0u - (mask >> j & 1);
-          *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * y + j][(16 * lane) ^ (16 * swizzle(j))]) =
-              codes_to_bf16(make_uint2(v.x & keep, v.y & keep));
+          *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * y + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
           if (j == 0 && lane < kOwn)
             sh.scl[in][kOwn * y + lane] = mask >> lane & 1 ? sh.raw_scale[in][kOwn * y + lane] : 0.f;
         }
       };
 
       if (count) {
+        if constexpr (kRuns) {
+          look_up(0);
+        } else {
 #pragma unroll
-        for (int n = 0; n < kEarly + 2; n++) look_up(n);
+          for (int n = 0; n < kAhead + 2; n++) look_up(n);
+        }
         loads_left<0>();
 #pragma unroll
         for (int n = 0; n < kEarly; n++) {
           masks |= address(n) << (8 * n);
 #pragma unroll
-          for (int j = 0; j < kLoads - 1; j++) bring(n, j);
+          for (int j = 0; j < kPairs; j++) bring(n, j);
         }
+        masks |= address(kEarly) << (8 * kEarly);
       }
       bring_queries();
       loads_left<0>();
       if (count) {
         if (kInt8) {
 #pragma unroll
-          for (int j = 0; j < kOwn; j++) convert(0, j, masks);
+          for (int j = 0; j < kOwn; j++) convert(0, j, codes_of(0, j), masks);
         } else {
           if ((masks & 0xff) != 0xff) zero_rows(0, masks);
         }
         masks >>= 8;   // of the blocks from 1
       }
-      if (w == kHalf && lane < 2) sh.flag[lane] = 0;
+      if (w == kHalf && lane < 2) sh.again[lane] = -1;
       wg_barrier();   // the queries, the first block's rows
       Acc acc[kLT][kRT];
 #pragma unroll
@@ -699,17 +785,20 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         // + 4 into the raw one of block n + 1 (converted in the iteration
         // before), and block n + 2 is converted
         const int into = kInt8 ? next : buf > 0 ? buf - 1 : kBufs - 1;
-        const uint32_t mask = address(n + kAhead);
-        if (n >= 0 && uniform(sh.flag[n & 1])) {
+        constexpr int kRead = 4, kGroups = kKeys / kDepth;
+        const int part = lane / kSize, pr = lane & (kSize - 1), c16 = lane & 15;
+        bf16x8 pb[kGroups][kRT], v[kPvSteps];
+        const int again = sh.again[n & 1];
+        auto weights = [&]() {
 #pragma unroll
-          for (int j = 0; j < kRT; j++) {
-            const float alpha = sh.alpha[n & 1][kSize * j + (lane & (kSize - 1))];
+          for (int t = 0; t < kGroups; t++)
 #pragma unroll
-            for (int i = 0; i < kLT; i++)
-#pragma unroll
-              for (int q = 0; q < kAcc; q++) acc[i][j][q] *= alpha;
-          }
-        }
+            for (int j = 0; j < kRT; j++) {
+              const int chunk = kDepth / 8 * t + part;
+              pb[t][j] = *reinterpret_cast<const bf16x8*>(sh.p[n & 1][kSize * j + pr] + 16 * (chunk ^ (pr >> 1 & 3)));
+            }
+        };
+        weights();   // (before block 0: not used)
         if constexpr (!kInt8) {
           // Keys that some row of the tile may not see: 0 * inf would put NaN
           // into that row.  A row that sees such a key has NaN from its logit.
@@ -726,8 +815,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         // ---- O^T += V^T P^T: V's operands are read some steps ahead; between
         // the steps come the loads of a later block and the conversion.  In
         // the iteration before block 0 the weights and the output are zero.
-        constexpr int kRead = 4, kGroups = kKeys / kDepth, kFirst = kPvSteps / 2;
-        const int part = lane / kSize, pr = lane & (kSize - 1), c16 = lane & 15;
         // a transposing read gives a lane its column (latent) of four rows (keys)
         const int tr_row = kBig ? 8 * (lane >> 5) + (c16 >> 2) : 4 * g + (c16 >> 2);
         const int tr_col = (kBig ? 2 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
@@ -748,64 +835,67 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           const i32x2 v1 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p1)));
           return __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
         };
-        bf16x8 pb[kGroups][kRT], v[kPvSteps];
         if (n >= 0) {
-#pragma unroll
-          for (int t = 0; t < kGroups; t++)
-#pragma unroll
-            for (int j = 0; j < kRT; j++) {
-              const int chunk = kDepth / 8 * t + part;
-              pb[t][j] = *reinterpret_cast<const bf16x8*>(sh.p[n & 1][kSize * j + pr] + 16 * (chunk ^ (pr >> 1 & 3)));
-            }
 #pragma unroll
           for (int u = 0; u < kRead; u++) v[u] = operand(u);
         }
-        auto between = [&](int u) {   // kPvSteps = 8: the loads and the conversion, in eighths
-          if constexpr (kInt8) {
-            convert(after, u, masks);
-            if (u < kLoads - 1) bring(into, u);
-          } else {
-            bring(into, u);
-            if (u == 7) bring(into, 8);
+        uint2 codes[kOwn];
+        if constexpr (kInt8) {
+#pragma unroll
+          for (int j = 0; j < kOwn; j++) codes[j] = codes_of(after, j);
+        }
+        if (n >= 0 && uniform(again) == n) {
+          wg_barrier();   // the maxima
+          wg_barrier();   // P
+          weights();
+#pragma unroll
+          for (int j = 0; j < kRT; j++) {
+            const float alpha = sh.alpha[kSize * j + pr];
+#pragma unroll
+            for (int i = 0; i < kLT; i++)
+#pragma unroll
+              for (int q = 0; q < kAcc; q++) acc[i][j][q] *= alpha;
           }
-          if (u == 7) look_up(n + kAhead + 2);
+        }
+        const bool group = kRuns && ((n + kAhead + 1) & 63) == 32;
+        if (group) look_up(n + kAhead + 1 + 32);
+        auto between = [&](int u) {   // kPvSteps = 8
+          if constexpr (kInt8) convert(after, u, codes[u], masks);
+          if (u < kPairs) bring(into, u);
+          if (u == 5 && !kRuns) look_up(n + kAhead + 3);
+          if (u == 6) masks |= address(n + kAhead + 1) << (kInt8 ? 24 : 16);
         };
         static_assert(kPvSteps == 8 && kOwn == 8, "a row a step");
-        auto steps = [&](int from, int to) {
-          if (n >= 0) {
+        if (n >= 0) {
 #pragma unroll
-            for (int u = 0; u < kPvSteps; u++)
-              if (u >= from && u < to) {
-                const int i = u % kLT, t = u / kLT;
-                if (u + kRead < kPvSteps) v[u + kRead] = operand(u + kRead);
+          for (int u = 0; u < kPvSteps; u++) {
+            const int i = u % kLT, t = u / kLT;
+            if (u + kRead < kPvSteps) v[u + kRead] = operand(u + kRead);
 #pragma unroll
-                for (int j = 0; j < kRT; j++) {
-                  if constexpr (kBig)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
-                  else
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
-                }
-                between(u);
-                __builtin_amdgcn_sched_barrier(0);
-              }
-          } else {
-#pragma unroll
-            for (int u = 0; u < kPvSteps; u++)
-              if (u >= from && u < to) between(u);
+            for (int j = 0; j < kRT; j++) {
+              if constexpr (kBig)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
+              else
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], pb[t][j], acc[i][j], 0, 0, 0);
+            }
+            between(u);
+            __builtin_amdgcn_sched_barrier(0);
           }
-        };
-        steps(0, kFirst);
-        wg_barrier();   // the maxima
-        if (w == kHalf && lane == 0) sh.flag[n & 1] = 0;   // (block n + 2 sets it after this iteration)
-        steps(kFirst, kPvSteps);
-        loads_left<kLoads>();   // all but this iteration's: block n + 2's rows (INT8: n + 3's) are there
+        } else {
+#pragma unroll
+          for (int u = 0; u < kPvSteps; u++) between(u);
+        }
+        // all but this iteration's: block n + 2's rows (INT8: n + 3's) are there
+        if (group)
+          loads_left<kLoads + 1>();
+        else
+          loads_left<kLoads>();
         if (!kInt8 && (masks & 0xff) != 0xff) zero_rows(after, masks);
-        masks = kInt8 ? masks >> 8 | mask << 8 : mask;   // from block n + 3 on
-        wg_barrier();   // P
+        masks >>= 8;   // from block n + 3 on
+        wg_barrier();    // P
         buf = next;
       }
       loads_left<0>();   // what was asked for past the last block
-      wg_barrier();
       wg_barrier();      // the sums
 
       // ---- the output as bf16 into LDS, or the partial
@@ -844,9 +934,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
                   f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
             }
         if (y == 0 && lane < kTM)
-          e->ml[static_cast<int64_t>(slot) * kTM + lane] = make_float2(sh.alpha[0][lane], sum_of(lane));
+          e->ml[static_cast<int64_t>(slot) * kTM + lane] = make_float2(sh.alpha[lane], sum_of(lane));
         if (lo <= start && y == 0 && lane == 0) {
-          const int64_t groups = min(static_cast<int>(gridDim.x), total);
           // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
           const int64_t last_unit = start + units;
           e->shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
@@ -874,7 +963,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         if (lse && lane == 0) {
           const float l = sh.red[0][j] + sh.red[1][j];
           lse[static_cast<int64_t>(rq.t0 + tok) * heads + head] =
-              l == 0.f ? -INFINITY : (sh.alpha[0][j] + __builtin_amdgcn_logf(l)) * kLn2;
+              l == 0.f ? -INFINITY : (sh.alpha[j] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
       if (kSplit && threadIdx.x == 0) e->shares[tile] = make_int2(-1, -1);
@@ -998,17 +1087,17 @@ Workspace workspace_of(int tm, int64_t tiles) {
   return w;
 }
 
-template <int kTM, bool kInt8>
+template <int kTM, bool kInt8, bool kRuns>
 int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
   if (a.num_tiles > kMaxSplitTiles) {
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false, kRuns>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true>), dim3(num_cus()), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a);
     // a shared tile has about CUs / tiles partials: 16 waves on a job where
     // that is many, one where it is few
     if (a.num_tiles <= 16)
@@ -1017,6 +1106,12 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
       hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 1>), dim3(kTM / 2, a.num_tiles), dim3(256), 0, st, a);
   }
   return static_cast<int>(hipGetLastError());
+}
+
+template <bool kInt8, bool kRuns>
+int launch_of(int tm, ChunkArgs& a, void* workspace, hipStream_t st) {
+  if (tm == 16) return launch<16, kInt8, kRuns>(a, workspace, st);
+  return tm == 32 ? launch<32, kInt8, kRuns>(a, workspace, st) : launch<64, kInt8, kRuns>(a, workspace, st);
 }
 
 }  // namespace
@@ -1079,18 +1174,15 @@ extern "C" int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h, const 
   a.div_sh1 = log2_block < 1 ? log2_block : 1, a.div_sh2 = log2_block > 1 ? log2_block - 1 : 0;
   a.num_reqs = static_cast<int>(num_reqs), a.total_q = static_cast<int>(total_q), a.heads = static_cast<int>(num_heads);
   a.num_tiles = static_cast<int>(tiles);
-  a.scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
-  // a scale of 0: the least that still leaves a masked logit -inf
-  if (a.scale_log2 == 0.f) a.scale_log2 = 1.17549435e-38f;
-  a.masked = a.scale_log2 >= 0.f ? -INFINITY : INFINITY;
+  const float scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
+  a.scale_log2 = fabsf(scale_log2);
+  a.flip = scale_log2 < 0.f ? 0x80008000u : 0;
   a.out = static_cast<uint16_t*>(out);
   a.so_t = so_t, a.so_h = so_h;
   a.out_align16 = oa % 16 == 0 && so_t % 8 == 0 && so_h % 8 == 0;
   a.lse = lse;
-  if (kv_is_int8) {
-    if (tm == 16) return launch<16, true>(a, workspace, st);
-    return tm == 32 ? launch<32, true>(a, workspace, st) : launch<64, true>(a, workspace, st);
-  }
-  if (tm == 16) return launch<16, false>(a, workspace, st);
-  return tm == 32 ? launch<32, false>(a, workspace, st) : launch<64, false>(a, workspace, st);
+  // (a row's offset from the first of eight is 32 bits)
+  const bool runs = block_size % kOwn == 0 && row_bytes < (INT64_C(1) << 28);
+  if (kv_is_int8) return runs ? launch_of<true, true>(tm, a, workspace, st) : launch_of<true, false>(tm, a, workspace, st);
+  return runs ? launch_of<false, true>(tm, a, workspace, st) : launch_of<false, false>(tm, a, workspace, st);
 }
