@@ -21,7 +21,7 @@
 //     each with the output in registers, and the loads.  bf16 rows come into a
 //     ring of four blocks in LDS by direct global -> LDS loads, three blocks
 //     ahead; INT8 rows as they are, four ahead, converted to bf16 once, two
-//     blocks before their use as V.  Nothing waits for memory but the count of
+//     blocks before their use as V, a half by each kind.  Nothing waits for memory but the count of
 //     outstanding loads, once a block: the block table's entries come ahead too.
 // The softmax goes against a row's reference, which stays until a logit passes
 // it by 2^16 (in the first block, and seldom after it): then the block is
@@ -47,8 +47,25 @@ constexpr int kLatent = 512;
 constexpr int kRope = 64;
 constexpr int kKeys = 32;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
+constexpr int kTileCost = 4;        // what starting and ending a tile costs, in blocks
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 16.f;      // how far (log2) a logit may pass its row's reference
+
+// n / d for any n, by multiplication.
+struct Divider {
+  uint32_t mul;
+  int sh1, sh2;
+};
+Divider divider(int64_t d) {
+  int log2_d = 0;   // rounded up
+  while ((INT64_C(1) << log2_d) < d) log2_d++;
+  const uint64_t mul = ((uint64_t(1) << log2_d) - static_cast<uint64_t>(d)) * (uint64_t(1) << 32) / static_cast<uint64_t>(d) + 1;
+  return {static_cast<uint32_t>(mul), log2_d < 1 ? log2_d : 1, log2_d > 1 ? log2_d - 1 : 0};
+}
+__device__ __forceinline__ int divide(uint32_t n, const Divider& d) {
+  const uint32_t t = __umulhi(d.mul, n);
+  return static_cast<int>((t + ((n - t) >> d.sh1)) >> d.sh2);
+}
 
 struct ChunkArgs {
   const uint16_t* q;
@@ -62,8 +79,7 @@ struct ChunkArgs {
   int64_t bt_stride;
   int max_blocks;
   int block_size;
-  uint32_t div_mul;   // position / block_size by multiplication (divide())
-  int div_sh1, div_sh2;
+  Divider by_block, by_heads;
   int num_reqs;
   int first_step;  // of a binary search over the requests: the largest power of two below num_reqs, or 0
   int total_q;
@@ -234,10 +250,10 @@ __device__ __forceinline__ int first_tile(int t0, int heads, int r) {
 
 // The last position that the tile's last row sees (-1: none), within the table.
 template <int kTM>
-__device__ __forceinline__ int last_key(const Request& r, int row0, int heads, int max_pos) {
+__device__ __forceinline__ int last_key(const Request& r, int row0, int heads, const Divider& by_heads, int max_pos) {
   const int rows = r.n * heads;
   const int last_row = min(row0 + kTM, rows) - 1;
-  const int64_t k = static_cast<int64_t>(r.len) - r.n + last_row / heads;
+  const int64_t k = static_cast<int64_t>(r.len) - r.n + divide(last_row, by_heads);
   return k < 0 ? -1 : static_cast<int>(k < max_pos ? k : max_pos - 1);
 }
 
@@ -248,11 +264,6 @@ __device__ __forceinline__ LateArgs* late_args() {
   uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return (LateArgs*)p;
-}
-
-__device__ __forceinline__ int divide(uint32_t n, uint32_t mul, int sh1, int sh2) {
-  const uint32_t t = __umulhi(mul, n);
-  return static_cast<int>((t + ((n - t) >> sh1)) >> sh2);
 }
 
 // kRuns: pages of a multiple of eight rows, so that the eight rows of a block
@@ -282,7 +293,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
   // ---- which blocks of which tiles are this workgroup's
-  int tile, lo = 0, hi = 0, total = 0, groups = 1;
+  int tile, lo = 0, hi = 0, each = 0, more = 0;   // the first `more` of the runs are each + 1 units long
   if (kSplit) {
     constexpr int kTiles = kMaxSplitTiles / kThreads;   // tiles of a thread
     int units[kTiles], req[kTiles], sum = 0;
@@ -306,7 +317,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       of[k] = rq;
       units[k] = 0;
       if (t < a.num_tiles && row0 >= 0 && row0 < rq.n * a.heads)
-        units[k] = max(1, last_key<kTM>(rq, row0, a.heads, max_pos) / kKeys + 1);
+        units[k] = kTileCost + max(1, last_key<kTM>(rq, row0, a.heads, a.by_heads, max_pos) / kKeys + 1);
       sum += units[k];
     }
     int upto = sum;                                     // inclusive scan over the wave
@@ -321,7 +332,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     if (lane == 63) sh.sums[w] = upto, sh.tiles[w] = filled;
     if (threadIdx.x == 0) sh.first = 0;
     wg_barrier();
-    int before = 0, tiles = 0;
+    int before = 0, tiles = 0, total = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; i++) {
       const int s = sh.sums[i];
@@ -339,10 +350,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     // read, joined) kTM / 512 of that: the sum of both is least with
     // sqrt(total * 512 / kTM) runs.  No fewer than tiles: those come without partials.
     const int best = max(tiles, static_cast<int>(sqrtf(static_cast<float>(total) * (512 / kTM))));
-    groups = min(min(static_cast<int>(gridDim.x), total), best);
-    if (static_cast<int>(blockIdx.x) >= groups) return;
-    lo = static_cast<int>(blockIdx.x * static_cast<int64_t>(total) / groups);
-    hi = static_cast<int>((blockIdx.x + 1) * static_cast<int64_t>(total) / groups);
+    const int groups = min(min(static_cast<int>(gridDim.x), total), best), g = blockIdx.x;
+    if (g >= groups) return;
+    each = static_cast<uint32_t>(total) / static_cast<uint32_t>(groups), more = total - each * groups;
+    lo = g * each + min(g, more), hi = lo + each + (g < more);
     int end = before + upto - sum;
 #pragma unroll
     for (int k = 0; k < kTiles; k++) {
@@ -363,17 +374,22 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   for (;; tile++) {
     asm volatile("" : "+v"(lane));   // nothing that depends on the lane alone is kept from tile to tile
     // ---- the tile: its request, its rows, its blocks [b0, b0 + count)
-    int r, b0 = 0, count = 0, start = 0, units = 0;
+    int r, b0 = 0, count = 0, last_unit = 0;
+    bool whole = true;
     if (kSplit) {
       if (tile >= kMaxSplitTiles) return;
-      start = tile ? uniform(sh.ends[tile - 1]) : 0;
+      const int start = tile ? uniform(sh.ends[tile - 1]) : 0;
       const int end = uniform(sh.ends[tile]);
       if (start >= hi) return;
-      units = end - start;
-      if (units == 0) continue;
+      if (start == end) continue;
+      // (its blocks come after kTileCost units that stand for its start and end)
+      const int first = start + kTileCost;
+      b0 = max(lo - first, 0);
+      count = min(hi, end) - first - b0;
+      if (count <= 0) continue;
+      last_unit = end - 1;
+      whole = b0 == 0 && count == end - first;
       r = uniform(sh.reqs[tile]);
-      b0 = max(lo - start, 0);
-      count = min(hi - start, units) - b0;
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
       int begun = 0;
@@ -396,13 +412,13 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
-    const int last = last_key<kTM>(rq, row0, a.heads, max_pos);
+    const int last = last_key<kTM>(rq, row0, a.heads, a.by_heads, max_pos);
     if (!kSplit)
       count = last >= 0 ? last / kKeys + 1 : 0;
     else if (last < 0)
       count = 0;   // nothing to see: its one unit writes the zeros
     // the least of the rows' last positions: keys past it are masked for some row
-    const int64_t least64 = static_cast<int64_t>(rq.len) - rq.n + row0 / a.heads;
+    const int64_t least64 = static_cast<int64_t>(rq.len) - rq.n + divide(row0, a.by_heads);
     const int least = static_cast<int>(least64 < -1 ? -1 : least64 < last ? least64 : last);
 
     if (kSplit) wg_barrier();   // LDS is free (the tile before, the scan)
@@ -413,10 +429,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     // The queries come through LDS, laid out like keys, in the ring's buffers
     // that the first blocks leave: wave w brings in every eighth row.
     constexpr int kQBuf = kInt8 ? 1 : 2;
+    constexpr int kMine = kTM / kWaves, kQueryLoads = kInt8 ? kMine : 2 * kMine;
     auto bring_queries = [&]() {
-      constexpr int kMine = kTM / kWaves;
       const int row = min(row0 + kWaves * min(c, kMine - 1) + w, rows - 1);   // (rows past the last: the last, not stored)
-      const int tok = row / a.heads, head = row - tok * a.heads;
+      const int tok = divide(row, a.by_heads), head = row - tok * a.heads;
       const uint64_t at = reinterpret_cast<uint64_t>(a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t +
                                                      static_cast<int64_t>(head) * a.sq_h);
       const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
@@ -432,6 +448,19 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           if (lane < 8) load_lds16(lds_offset(qs.rope[key & 31]), from, 2 * kLatent + 16 * (lane ^ swizzle(key)));
         }
       }
+    };
+
+    // INT8: row 8 z + j of raw block `in`, and as bf16 into the block there
+    // (without a row: any codes, with the scale 0)
+    auto codes_of = [&](int in, int z, int j) {
+      if constexpr (kInt8)
+        return *reinterpret_cast<const uint2*>(&sh.raw[in][kOwn * z + j][8 * lane]);
+      else
+        return make_uint2(0, 0);
+    };
+    auto convert = [&](int in, int z, int j, uint2 v) {
+      if constexpr (kInt8)
+        *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * z + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
     };
 
     if (w < kHalf) {
@@ -535,7 +564,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
         for (int rt = 0; rt < kRQ; rt++) sum[rt] += part_sum[rt];
         if (n == count) break;
-        if (takes_rows) {
+        // INT8: half of the next block's conversion, between the products
+        const int next = buf + 1 < kBufs ? buf + 1 : 0;
+        uint2 codes[kOwn / 2];
+#pragma unroll
+        for (int j = 0; j < kOwn / 2; j++) codes[j] = codes_of(next, w, kOwn / 2 + j);
+        if (!takes_rows) {
+#pragma unroll
+          for (int j = 0; j < kOwn / 2; j++) convert(next, w, kOwn / 2 + j, codes[j]);
+        } else {
           const uint32_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v)));
           if constexpr (kInt8) {
             const float4 v = *reinterpret_cast<const float4*>(&sh.scl[buf][16 * kh + 4 * g]);
@@ -554,6 +591,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++)
               t[rt][st % kSums] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], t[rt][st % kSums], 0, 0, 0);
+            if (st % 4 == 1 && st / 4 < kOwn / 2) convert(next, w, kOwn / 2 + st / 4, codes[st / 4]);
             __builtin_amdgcn_sched_barrier(0);
           }
           float scale[4];
@@ -568,7 +606,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++) {
               const int row = min(row0 + 16 * (rh * kRQ + rt) + c, rows - 1);
-              const int64_t see = static_cast<int64_t>(rq.len) - rq.n + row / a.heads;
+              const int64_t see = static_cast<int64_t>(rq.len) - rq.n + divide(row, a.by_heads);
               const int limit = static_cast<int>(see < last ? see < -1 ? -1 : see : last) - (b0 + n) * kKeys;
 #pragma unroll
               for (int i = 0; i < 4; i++) {
@@ -591,7 +629,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           weigh(n);
         }
         wg_barrier();   // P
-        buf = buf + 1 < kBufs ? buf + 1 : 0;
+        buf = next;
       }
       if (count) wg_barrier();   // PV has read P and the rescaling for the last time
       if (takes_rows) {
@@ -620,7 +658,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       const int32_t* bt = a.bt + static_cast<int64_t>(r) * a.bt_stride;
       auto look_up = [&](int n) {       // the table's entries for block n, kRuns: for blocks n .. n + 63
         const int64_t at = kRuns ? (b0 + n + lane) * static_cast<int64_t>(kKeys) + kOwn * y : (b0 + n) * kKeys + (lane & 31);
-        const int pg = divide(static_cast<int>(at < last ? at : last), a.div_mul, a.div_sh1, a.div_sh2);
+        const int pg = divide(static_cast<int>(at < last ? at : last), a.by_block);
         if constexpr (kRuns) {
           load_lds4_at(lds_offset(&sh.page[64 * y]), bt + pg);
         } else {
@@ -651,7 +689,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           if ((n & 63) == 0) pages = sh.page[64 * y + lane];
           const uint32_t page = static_cast<uint32_t>(__builtin_amdgcn_readlane(pages, n & 63));
           const int pos = (b0 + n) * kKeys + kOwn * y;
-          const uint32_t in_page = static_cast<uint32_t>(pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size);
+          const uint32_t in_page = static_cast<uint32_t>(pos - divide(pos, a.by_block) * a.block_size);
           const int left = n < count && page < static_cast<uint32_t>(a.num_blocks) ? last - pos + 1 : 0;
           mask = left >= kOwn ? 0xffu : left > 0 ? (1u << left) - 1 : 0u;
           run = reinterpret_cast<uint64_t>(a.kv) +
@@ -659,7 +697,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         } else {
           const int key = kOwn * y + of_lane, pos = (b0 + n) * kKeys + key;
           const int page = sh.page[32 * (n & 7) + key];
-          const int in_page = pos - divide(pos, a.div_mul, a.div_sh1, a.div_sh2) * a.block_size;
+          const int in_page = pos - divide(pos, a.by_block) * a.block_size;
           const bool ok = n < count && pos <= last && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks);
           const uint64_t at = reinterpret_cast<uint64_t>(a.kv) +
                               (ok ? page * static_cast<uint64_t>(a.page_bytes) + in_page * static_cast<uint64_t>(a.row_bytes) : 0);
@@ -723,18 +761,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             }
         }
       };
-      // INT8: row j of the wave's in raw block `in`, and as bf16 into the block
-      // there (without a row: any codes, with the scale 0)
-      auto codes_of = [&](int in, int j) {
-        if constexpr (kInt8)
-          return *reinterpret_cast<const uint2*>(&sh.raw[in][kOwn * y + j][8 * lane]);
-        else
-          return make_uint2(0, 0);
-      };
-      auto convert = [&](int in, int j, uint2 v, uint32_t mask) {
+      auto scales = [&](int in, uint32_t mask) {
         if constexpr (kInt8) {
-          *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * y + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
-          if (j == 0 && lane < kOwn)
+          if (lane < kOwn)
             sh.scl[in][kOwn * y + lane] = mask >> lane & 1 ? sh.raw_scale[in][kOwn * y + lane] : 0.f;
         }
       };
@@ -746,7 +775,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
           for (int n = 0; n < kAhead + 2; n++) look_up(n);
         }
-        loads_left<0>();
+      }
+      bring_queries();
+      if (count) {
+        loads_left<kQueryLoads>();
 #pragma unroll
         for (int n = 0; n < kEarly; n++) {
           masks |= address(n) << (8 * n);
@@ -754,17 +786,17 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           for (int j = 0; j < kPairs; j++) bring(n, j);
         }
         masks |= address(kEarly) << (8 * kEarly);
-      }
-      bring_queries();
-      loads_left<0>();
-      if (count) {
+        loads_left<kRowLoads>();   // the last of these blocks may be on its way
         if (kInt8) {
 #pragma unroll
-          for (int j = 0; j < kOwn; j++) convert(0, j, codes_of(0, j), masks);
+          for (int j = 0; j < kOwn; j++) convert(0, y, j, codes_of(0, y, j));
+          scales(0, masks);
         } else {
           if ((masks & 0xff) != 0xff) zero_rows(0, masks);
         }
         masks >>= 8;   // of the blocks from 1
+      } else {
+        loads_left<0>();
       }
       if (w == kHalf && lane < 2) sh.again[lane] = -1;
       wg_barrier();   // the queries, the first block's rows
@@ -839,11 +871,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
           for (int u = 0; u < kRead; u++) v[u] = operand(u);
         }
-        uint2 codes[kOwn];
-        if constexpr (kInt8) {
+        uint2 codes[kOwn / 2];
 #pragma unroll
-          for (int j = 0; j < kOwn; j++) codes[j] = codes_of(after, j);
-        }
+        for (int j = 0; j < kOwn / 2; j++) codes[j] = codes_of(after, y, j);
         if (n >= 0 && uniform(again) == n) {
           wg_barrier();   // the maxima
           wg_barrier();   // P
@@ -860,7 +890,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         const bool group = kRuns && ((n + kAhead + 1) & 63) == 32;
         if (group) look_up(n + kAhead + 1 + 32);
         auto between = [&](int u) {   // kPvSteps = 8
-          if constexpr (kInt8) convert(after, u, codes[u], masks);
+          if (u < kOwn / 2) convert(after, y, u, codes[u]);
+          if (u == kOwn / 2) scales(after, masks);
           if (u < kPairs) bring(into, u);
           if (u == 5 && !kRuns) look_up(n + kAhead + 3);
           if (u == 6) masks |= address(n + kAhead + 1) << (kInt8 ? 24 : 16);
@@ -901,7 +932,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       // ---- the output as bf16 into LDS, or the partial
       auto sum_of = [&](int row) { return sh.red[0][row] + sh.red[1][row]; };
       const int part = lane / kSize, pr = lane & (kSize - 1);
-      if (!kSplit || (lo <= start && start + units <= hi)) {
+      if (whole) {
         // chunk c of 16 bytes of row r at c ^ (r % 8), so that rows fall on different banks
         uint8_t* os = sh.kv[0].lat[0];
 #pragma unroll
@@ -921,7 +952,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       } else {
         // slot 2 g: the tile began in an earlier workgroup; 2 g + 1: it begins
         // here.  In the accumulators' order: 16 bytes of each lane at a time.
-        const int slot = 2 * static_cast<int>(blockIdx.x) + (lo <= start);
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (b0 == 0);
         float* out = e->part + static_cast<int64_t>(slot) * (kTM * kLatent);
 #pragma unroll
         for (int i = 0; i < kLT; i++)
@@ -935,23 +966,23 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             }
         if (y == 0 && lane < kTM)
           e->ml[static_cast<int64_t>(slot) * kTM + lane] = make_float2(sh.alpha[lane], sum_of(lane));
-        if (lo <= start && y == 0 && lane == 0) {
-          // the workgroup of the tile's last unit u: the largest g with g * total / groups <= u
-          const int64_t last_unit = start + units;
-          e->shares[tile] = make_int2(blockIdx.x, static_cast<int>((last_unit * groups - 1) / total));
+        if (b0 == 0 && y == 0 && lane == 0) {
+          const int longer = more * (each + 1);   // units of the longer runs
+          e->shares[tile] = make_int2(blockIdx.x, last_unit < longer ? last_unit / (each + 1) : more + (last_unit - longer) / each);
         }
       }
     }
 
-    if (!kSplit || (lo <= start && start + units <= hi)) {   // whole rows go out, every eighth of each wave's
+    if (whole) {   // whole rows go out, every eighth of each wave's
       wg_barrier();
       const uint8_t* os = sh.kv[0].lat[0];
       const int heads = e->heads, aligned = e->out_align16;
+      const Divider by_heads = {e->by_heads.mul, e->by_heads.sh1, e->by_heads.sh2};
       const int64_t so_t = e->so_t, so_h = e->so_h;
       uint16_t* out = e->out;
       float* lse = e->lse;
       for (int j = w; j < kTM && row0 + j < rows; j += kWaves) {
-        const int row = row0 + j, tok = row / heads, head = row - tok * heads;
+        const int row = row0 + j, tok = divide(row, by_heads), head = row - tok * heads;
         uint16_t* o = out + static_cast<int64_t>(rq.t0 + tok) * so_t + static_cast<int64_t>(head) * so_h;
         const uint4 v = *reinterpret_cast<const uint4*>(os + j * 2 * kLatent + ((16 * lane) ^ (16 * (j & 7))));
         if (aligned) {
@@ -1053,7 +1084,7 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
   const Request rq = request_of(a.cu[at], a.cu[at + 1], 0, a.total_q);
   const int row = (tile - first_tile<kTM>(rq.t0, a.heads, at)) * kTM + kRowSize * j + c;
   if (row >= rq.n * a.heads) return;
-  const int tok = row / a.heads, head = row - tok * a.heads;
+  const int tok = divide(row, a.by_heads), head = row - tok * a.heads;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* o = a.out + static_cast<int64_t>(rq.t0 + tok) * a.so_t + static_cast<int64_t>(head) * a.so_h;
   *reinterpret_cast<uint2*>(o + lat) =
@@ -1089,7 +1120,9 @@ Workspace workspace_of(int tm, int64_t tiles) {
 
 template <int kTM, bool kInt8, bool kRuns>
 int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
-  if (a.num_tiles > kMaxSplitTiles) {
+  // (units of all tiles are counted in an int)
+  const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.block_size;
+  if (a.num_tiles > kMaxSplitTiles || (cap / kKeys + 1 + kTileCost) * a.num_tiles > 0x7fffffff) {
     hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false, kRuns>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
@@ -1167,11 +1200,7 @@ extern "C" int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h, const 
   a.block_size = static_cast<int>(block_size);
   while (a.first_step < num_reqs && (a.first_step ? 2 * a.first_step : 1) < num_reqs)
     a.first_step = a.first_step ? 2 * a.first_step : 1;
-  int log2_block = 0;   // rounded up
-  while ((INT64_C(1) << log2_block) < block_size) log2_block++;
-  a.div_mul = static_cast<uint32_t>(((uint64_t(1) << log2_block) - static_cast<uint64_t>(block_size)) *
-                                        (uint64_t(1) << 32) / static_cast<uint64_t>(block_size) + 1);
-  a.div_sh1 = log2_block < 1 ? log2_block : 1, a.div_sh2 = log2_block > 1 ? log2_block - 1 : 0;
+  a.by_block = divider(block_size), a.by_heads = divider(num_heads);
   a.num_reqs = static_cast<int>(num_reqs), a.total_q = static_cast<int>(total_q), a.heads = static_cast<int>(num_heads);
   a.num_tiles = static_cast<int>(tiles);
   const float scale_log2 = static_cast<float>(sm_scale * 1.4426950408889634);
