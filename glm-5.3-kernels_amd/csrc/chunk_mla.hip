@@ -47,7 +47,7 @@ constexpr int kLatent = 512;
 constexpr int kRope = 64;
 constexpr int kKeys = 32;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
-constexpr int kTileCost = 4;        // what starting and ending a tile costs, in blocks
+constexpr int kTileCost = 10;       // what starting and ending a tile costs, in blocks
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 16.f;      // how far (log2) a logit may pass its row's reference
 
@@ -132,7 +132,9 @@ struct __attribute__((aligned(16))) ChunkShared {
   uint8_t have[8][kHalf];              // bit j of byte y: key 8 y + j of the block has a row
   int again[2];                        // the last (odd, even) block that is weighted again
   int sums[kWaves], tiles[kWaves];
-  int first, first_t0, first_n, first_len;   // the first tile and its request
+  struct __attribute__((aligned(16))) {
+    int tile, start, end, req, t0, n, len;
+  } first;                             // the first tile, its units and its request
 };
 
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -293,6 +295,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
   const int max_pos = static_cast<int>(cap < 0x7fffff00 ? cap : 0x7fffff00);   // a block's positions stay ints
 
   // ---- which blocks of which tiles are this workgroup's
+  int r = 0, start = 0, end = 0;   // the tile's request and units
+  Request rq = {};
   int tile, lo = 0, hi = 0, each = 0, more = 0;   // the first `more` of the runs are each + 1 units long
   if (kSplit) {
     constexpr int kTiles = kMaxSplitTiles / kThreads;   // tiles of a thread
@@ -330,7 +334,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
     for (int k = 0; k < kTiles; k++) filled += __popcll(__ballot(units[k] > 0));
     if (lane == 63) sh.sums[w] = upto, sh.tiles[w] = filled;
-    if (threadIdx.x == 0) sh.first = 0;
     wg_barrier();
     int before = 0, tiles = 0, total = 0;
 #pragma unroll
@@ -347,39 +350,42 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       return;   // uniform over the workgroup
     }
     // A run of u blocks takes u times a block's time, and its partial (written,
-    // read, joined) kTM / 512 of that: the sum of both is least with
-    // sqrt(total * 512 / kTM) runs.  No fewer than tiles: those come without partials.
-    const int best = max(tiles, static_cast<int>(sqrtf(static_cast<float>(total) * (512 / kTM))));
+    // read, joined) kTM / 1024 of that: the sum of both is least with
+    // sqrt(total * 1024 / kTM) runs.  No fewer than tiles: those come without partials.
+    const int best = max(tiles, static_cast<int>(sqrtf(static_cast<float>(total) * (1024 / kTM))));
     const int groups = min(min(static_cast<int>(gridDim.x), total), best), g = blockIdx.x;
     if (g >= groups) return;
     each = static_cast<uint32_t>(total) / static_cast<uint32_t>(groups), more = total - each * groups;
     lo = g * each + min(g, more), hi = lo + each + (g < more);
-    int end = before + upto - sum;
+    int upto_t = before + upto - sum;
 #pragma unroll
     for (int k = 0; k < kTiles; k++) {
       const int t = static_cast<int>(threadIdx.x) * kTiles + k;
-      if (end <= lo && lo < end + units[k])
-        sh.first = t, sh.first_t0 = of[k].t0, sh.first_n = of[k].n, sh.first_len = of[k].len;
-      end += units[k];
-      sh.ends[t] = end;
+      if (upto_t <= lo && lo < upto_t + units[k])
+        sh.first = {t, upto_t, upto_t + units[k], req[k], of[k].t0, of[k].n, of[k].len};
+      upto_t += units[k];
+      sh.ends[t] = upto_t;
       sh.reqs[t] = req[k];
       if (blockIdx.x == 0 && t < a.num_tiles && units[k] == 0) a.shares[t] = make_int2(-1, -1);
     }
     wg_barrier();
-    tile = uniform(sh.first);
+    const auto first = sh.first;
+    tile = uniform(first.tile), start = uniform(first.start), end = uniform(first.end), r = uniform(first.req);
+    rq = {uniform(first.t0), uniform(first.n), uniform(first.len)};
   } else {
     tile = a.num_tiles - 1 - static_cast<int>(blockIdx.x);
   }
 
-  for (;; tile++) {
+  for (bool known = kSplit;; tile++, known = false) {
     asm volatile("" : "+v"(lane));   // nothing that depends on the lane alone is kept from tile to tile
     // ---- the tile: its request, its rows, its blocks [b0, b0 + count)
-    int r, b0 = 0, count = 0, last_unit = 0;
+    int b0 = 0, count = 0, last_unit = 0;
     bool whole = true;
     if (kSplit) {
-      if (tile >= kMaxSplitTiles) return;
-      const int start = tile ? uniform(sh.ends[tile - 1]) : 0;
-      const int end = uniform(sh.ends[tile]);
+      if (!known) {
+        if (tile >= kMaxSplitTiles) return;
+        start = end, end = uniform(sh.ends[tile]), r = uniform(sh.reqs[tile]);
+      }
       if (start >= hi) return;
       if (start == end) continue;
       // (its blocks come after kTileCost units that stand for its start and end)
@@ -389,7 +395,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       if (count <= 0) continue;
       last_unit = end - 1;
       whole = b0 == 0 && count == end - first;
-      r = uniform(sh.reqs[tile]);
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
       int begun = 0;
@@ -404,11 +409,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       for (int i = 0; i < kWaves; i++) r += sh.sums[i];
       r = uniform(max(r, 0));
     }
-    Request rq;
-    if (kSplit && tile == uniform(sh.first))
-      rq = {uniform(sh.first_t0), uniform(sh.first_n), uniform(sh.first_len)};
-    else
-      rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
+    if (!known) rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
@@ -1131,10 +1132,13 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
     hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a);
-    // a shared tile has about CUs / tiles partials: 16 waves on a job where
-    // that is many, one where it is few
-    if (a.num_tiles <= 16)
+    // a shared tile has at most about CUs / tiles partials: 16 waves on a job
+    // where that is many, four or one where it is few
+    const int partials = num_cus() / a.num_tiles;
+    if (partials > 64)
       hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 16>), dim3(2 * kTM, a.num_tiles), dim3(1024), 0, st, a);
+    else if (partials > 24)
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 4>), dim3(2 * kTM, a.num_tiles), dim3(256), 0, st, a);
     else
       hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 1>), dim3(kTM / 2, a.num_tiles), dim3(256), 0, st, a);
   }
