@@ -114,7 +114,7 @@ struct __attribute__((aligned(16))) ChunkShared {
   static constexpr int kBufs = kInt8 ? 3 : 4;
   struct __attribute__((aligned(16))) Bf16Block {
     uint8_t lat[kKeys][2 * kLatent];   // chunk c of 16 bytes of row k at chunk c ^ swizzle(k)
-    uint8_t rope[kKeys][2 * kRope];
+    uint8_t rope[kKeys][2 * kRope];    // chunk c of row k at chunk c ^ rope_swizzle(k)
   };
   struct __attribute__((aligned(16))) Int8Block {
     uint8_t lat[kKeys][2 * kLatent];
@@ -123,7 +123,7 @@ struct __attribute__((aligned(16))) ChunkShared {
   uint8_t raw[kInt8 ? 3 : 0][kKeys][kLatent];   // INT8 rows as they are in the cache
   float raw_scale[kInt8 ? 3 : 0][kKeys];
   float scl[kInt8 ? 3 : 0][kKeys];              // the scales, 0 for a key without a row
-  uint8_t p[2][kTM][2 * kKeys];        // P, chunk c of 16 bytes of row r at c ^ (r / 2 % 4)
+  uint8_t p[2][kTM][2 * kKeys];        // P, chunk c of 16 bytes of row r at c ^ (r / 4 % 4)
   int32_t page[kHalf * 64];            // block table entries of the coming blocks
   float red[2][kTM];                   // per key half: maxima; at the end the sums
   float alpha[kTM];                    // what new references scale the output with; at the end the references
@@ -178,11 +178,13 @@ __device__ __forceinline__ void load_lds4_at(uint32_t dst, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(p) : "memory");
 }
 
-// Swizzle of a row's 16-byte chunks (on the low three bits of the chunk's
-// index).  Eight lanes that read one chunk of rows 0..7 (the K operand, a
-// 128-byte pass) meet eight different chunk columns; four rows 4g .. 4g + 3
-// of a transposing read (two neighbouring chunks each) four different pairs.
-__device__ __forceinline__ int swizzle(int key) { return ((key & 3) << 1) | ((key >> 2) & 1); }
+// Swizzles of a row's 16-byte chunks, on the low bits of the chunk's index, for
+// LDS passes of 256 bytes.  Sixteen lanes that read one chunk of rows 0 .. 15
+// (the K operand) meet sixteen different chunk columns; the transposing reads
+// (four rows of four chunks each, or eight of two) meet different fours or pairs.
+__device__ __forceinline__ int swizzle(int key) { return (key & 3) << 2 | (key >> 1 & 2) | (key >> 3 & 1); }
+// Rotary parts are 128 bytes: two rows a pass's width.
+__device__ __forceinline__ int rope_swizzle(int key) { return key >> 1 & 7; }
 
 // Maximum and sum over a row's lanes: four of 16 apart (quad), two of 32 (half).
 __device__ __forceinline__ float quad_max(float v) {
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         auto& qs = sh.kv[kQBuf + (key >> 5)];
         load_lds16(lds_offset(qs.lat[key & 31]), from, 16 * (lane ^ swizzle(key)));
         if constexpr (!kInt8) {
-          if (lane < 8) load_lds16(lds_offset(qs.rope[key & 31]), from, 2 * kLatent + 16 * (lane ^ swizzle(key)));
+          if (lane < 8) load_lds16(lds_offset(qs.rope[key & 31]), from, 2 * kLatent + 16 * (lane ^ rope_swizzle(key)));
         }
       }
     };
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     };
     auto convert = [&](int in, int z, int j, uint2 v) {
       if constexpr (kInt8)
-        *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * z + j][(16 * lane) ^ (16 * swizzle(j))]) = codes_to_bf16(v);
+        *reinterpret_cast<uint4*>(&sh.kv[in].lat[kOwn * z + j][(16 * lane) ^ (16 * swizzle(kOwn * z + j))]) = codes_to_bf16(v);
     };
 
     if (w < kHalf) {
@@ -478,9 +480,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         const auto& qs = sh.kv[kQBuf + (key >> 5)];
 #pragma unroll
         for (int st = 0; st < kSteps; st++) {
-          const uint8_t* from = qs.lat[key & 31] + 16 * ((4 * (st & 1) + g) ^ sw) + 128 * (st >> 1);
+          const uint8_t* from = qs.lat[key & 31] + 16 * ((4 * (st & 3) + g) ^ sw) + 256 * (st >> 2);
           if constexpr (!kInt8) {
-            if (st >= 16) from = qs.rope[key & 31] + 16 * ((4 * (st - 16) + g) ^ sw);
+            if (st >= 16) from = qs.rope[key & 31] + 16 * ((4 * (st - 16) + g) ^ rope_swizzle(c));
           }
           const uint4 v = *reinterpret_cast<const uint4*>(from);
           qf[rt][st] = __builtin_bit_cast(bf16x8, make_uint4(v.x ^ a.flip, v.y ^ a.flip, v.z ^ a.flip, v.w ^ a.flip));
@@ -510,7 +512,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           // the average); the sum keeps the unrounded weights.  With the
           // small products of PV the operand's keys are 4 g + i, 16 + 4 g + i.
           const int chunk = kBig ? 2 * kh + (g >> 1) : g, half = kBig ? g & 1 : kh;
-          *reinterpret_cast<uint2*>(sh.p[n & 1][16 * (rh * kRQ + rt) + c] + 16 * (chunk ^ (c >> 1 & 3)) + 8 * half) =
+          *reinterpret_cast<uint2*>(sh.p[n & 1][16 * (rh * kRQ + rt) + c] + 16 * (chunk ^ (c >> 2 & 3)) + 8 * half) =
               make_uint2(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]));
         }
       };
@@ -521,12 +523,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         constexpr int kRead = 6;
         const int key = 16 * kh + c, sw = swizzle(c);
         const auto& blk = sh.kv[buf];
-        const uint8_t* even = blk.lat[key] + 16 * (g ^ sw);
-        const uint8_t* odd = blk.lat[key] + 16 * ((4 + g) ^ sw);
         auto operand = [&](int st) {
-          const uint8_t* from = (st & 1 ? odd : even) + 128 * (st >> 1);
+          const uint8_t* from = blk.lat[key] + 16 * ((4 * (st & 3) + g) ^ sw) + 256 * (st >> 2);
           if constexpr (!kInt8) {
-            if (st >= 16) from = blk.rope[key] + 16 * ((4 * (st - 16) + g) ^ sw);
+            if (st >= 16) from = blk.rope[key] + 16 * ((4 * (st - 16) + g) ^ rope_swizzle(c));
           }
           return *reinterpret_cast<const bf16x8*>(from);
         };
@@ -678,8 +678,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           if (kInt8)
             row_off[j] = j < 4 ? (2 * j + (lane >> 5)) * rb + 16 * (lane & 31) : (lane & 7) * rb + kLatent;
           else
-            row_off[j] = j < kOwn ? j * rb + ((16 * lane) ^ (16 * swizzle(j)))
-                                  : (lane >> 3) * rb + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3));
+            row_off[j] = j < kOwn ? j * rb + ((16 * lane) ^ (16 * swizzle(kOwn * y + j)))
+                                  : (lane >> 3) * rb + 2 * kLatent + 16 * ((lane & 7) ^ rope_swizzle(kOwn * y + (lane >> 3)));
         }
       }
       const int of_lane = kInt8 ? lane & 7 : lane >> 3;
@@ -744,12 +744,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             if constexpr (kRuns)
               load_lds16(lds_offset(sh.kv[to].rope[kOwn * y]), base, row_off[kRowLoads - 1]);
             else
-              load_lds16_at(lds_offset(sh.kv[to].rope[kOwn * y]), own + 2 * kLatent + 16 * ((lane & 7) ^ swizzle(lane >> 3)));
+              load_lds16_at(lds_offset(sh.kv[to].rope[kOwn * y]), own + 2 * kLatent + 16 * ((lane & 7) ^ rope_swizzle(kOwn * y + (lane >> 3))));
           } else if constexpr (kRuns) {
             load_lds16_2(dst, base, row_off[2 * j], row_off[2 * j + 1]);
           } else {
             for (int i = 0; i < 2; i++)
-              load_lds16(dst + 1024 * i, reinterpret_cast<const uint8_t*>(row_of(2 * j + i)), (16 * lane) ^ (16 * swizzle(2 * j + i)));
+              load_lds16(dst + 1024 * i, reinterpret_cast<const uint8_t*>(row_of(2 * j + i)), (16 * lane) ^ (16 * swizzle(kOwn * y + 2 * j + i)));
           }
         }
       };
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int j = 0; j < kRT; j++) {
               const int chunk = kDepth / 8 * t + part;
-              pb[t][j] = *reinterpret_cast<const bf16x8*>(sh.p[n & 1][kSize * j + pr] + 16 * (chunk ^ (pr >> 1 & 3)));
+              pb[t][j] = *reinterpret_cast<const bf16x8*>(sh.p[n & 1][kSize * j + pr] + 16 * (chunk ^ (pr >> 2 & 3)));
             }
         };
         weights();   // (before block 0: not used)
@@ -851,19 +851,17 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         // a transposing read gives a lane its column (latent) of four rows (keys)
         const int tr_row = kBig ? 8 * (lane >> 5) + (c16 >> 2) : 4 * g + (c16 >> 2);
         const int tr_col = (kBig ? 2 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
-        constexpr int kTileChunks = kSize / 8, kBases = 8 / kTileChunks;     // the swizzle is on 8 chunks
-        const uint8_t* base[kBases][kBig ? 2 : 1];
+        const uint8_t* base[kLT][kBig ? 2 : 1];
 #pragma unroll
-        for (int i = 0; i < kBases; i++)
+        for (int i = 0; i < kLT; i++)
 #pragma unroll
           for (int h = 0; h < (kBig ? 2 : 1); h++)
-            base[i][h] = &sh.kv[buf].lat[tr_row + 4 * h][256 * y + 16 * ((kTileChunks * i + tr_col) ^ swizzle(tr_row + 4 * h)) +
+            base[i][h] = &sh.kv[buf].lat[tr_row + 4 * h][256 * y + 16 * ((kSize / 8 * i + tr_col) ^ swizzle(tr_row + 4 * h)) +
                                                          8 * (c16 & 1)];
         auto operand = [&](int u) {
           const int i = u % kLT, t = u / kLT;   // latent tile, keys
-          const int off = 128 * (i / kBases) + kDepth * t * 2 * kLatent;
-          const uint8_t* p0 = base[i % kBases][0] + off;
-          const uint8_t* p1 = kBig ? base[i % kBases][kBig ? 1 : 0] + off : p0 + 16 * 2 * kLatent;
+          const uint8_t* p0 = base[i][0] + kDepth * t * 2 * kLatent;
+          const uint8_t* p1 = kBig ? base[i][kBig ? 1 : 0] + kDepth * t * 2 * kLatent : p0 + 16 * 2 * kLatent;
           const i32x2 v0 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p0)));
           const i32x2 v1 = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(GLM53_LDS(i16x4, p1)));
           return __builtin_bit_cast(bf16x8, make_uint4(v0[0], v0[1], v1[0], v1[1]));
@@ -934,7 +932,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       auto sum_of = [&](int row) { return sh.red[0][row] + sh.red[1][row]; };
       const int part = lane / kSize, pr = lane & (kSize - 1);
       if (whole) {
-        // chunk c of 16 bytes of row r at c ^ (r % 8), so that rows fall on different banks
+        // chunk c of 16 bytes of row r at c ^ (r % 16), so that rows fall on different banks
         uint8_t* os = sh.kv[0].lat[0];
 #pragma unroll
         for (int j = 0; j < kRT; j++) {
@@ -946,7 +944,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
             for (int q = 0; q < kAcc; q += 4) {
               const Acc v = acc[i][j];
               const int lat = 128 * y + kSize * i + 2 * q + 4 * part;   // of v[q]
-              *reinterpret_cast<uint2*>(os + (kSize * j + pr) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (pr & 7))) + (2 * lat & 15)) =
+              *reinterpret_cast<uint2*>(os + (kSize * j + pr) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (pr & 15))) + (2 * lat & 15)) =
                   make_uint2(pack_bf16x2(v[q] * inv, v[q + 1] * inv), pack_bf16x2(v[q + 2] * inv, v[q + 3] * inv));
             }
         }
@@ -985,7 +983,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       for (int j = w; j < kTM && row0 + j < rows; j += kWaves) {
         const int row = row0 + j, tok = divide(row, by_heads), head = row - tok * heads;
         uint16_t* o = out + static_cast<int64_t>(rq.t0 + tok) * so_t + static_cast<int64_t>(head) * so_h;
-        const uint4 v = *reinterpret_cast<const uint4*>(os + j * 2 * kLatent + ((16 * lane) ^ (16 * (j & 7))));
+        const uint4 v = *reinterpret_cast<const uint4*>(os + j * 2 * kLatent + ((16 * lane) ^ (16 * (j & 15))));
         if (aligned) {
           reinterpret_cast<uint4*>(o)[lane] = v;
         } else {
