@@ -109,6 +109,9 @@ struct ChunkShape {
   static constexpr bool kBig = kTM >= 32;
 };
 
+// Row m of wave y's latent tile i: tiles of 32 are two runs of 16, 64 apart.
+__device__ __forceinline__ int latent_of(int y, int i, int m) { return 128 * y + 16 * i + (m & 15) + 64 * (m >> 4); }
+
 template <int kTM, bool kInt8>
 struct __attribute__((aligned(16))) ChunkShared {
   static constexpr int kBufs = kInt8 ? 3 : 4;
@@ -179,10 +182,18 @@ __device__ __forceinline__ void load_lds4_at(uint32_t dst, const void* p) {
 }
 
 // Swizzles of a row's 16-byte chunks, on the low bits of the chunk's index, for
-// LDS passes of 256 bytes.  Sixteen lanes that read one chunk of rows 0 .. 15
-// (the K operand) meet sixteen different chunk columns; the transposing reads
-// (four rows of four chunks each, or eight of two) meet different fours or pairs.
-__device__ __forceinline__ int swizzle(int key) { return (key & 3) << 2 | (key >> 1 & 2) | (key >> 3 & 1); }
+// LDS passes of 256 bytes.  The row's place among its four, i, goes to bits 1
+// and 2, its four q to bits 3 and 0:
+//   * a transposing read takes pairs of chunks of four rows, of 32 lanes either
+//     both pairs (eight chunks apart) of one q or the same pair of two q's
+//     (0 and 1, or 2 and 3): i, the pair's bit 3 and q's bit 3 tell them apart;
+//   * the K operand's 16-byte reads take chunk 4 k + g of row 4 q + i in lane
+//     16 g + 4 q + i, and a pass serves lanes of q = 0, 3 and, from the next g,
+//     1, 2 (or the reverse): g differs in bit 0, where only 0 and 3, and only 1
+//     and 2, differ.
+__device__ __forceinline__ int swizzle(int key) {
+  return ((key >> 2 ^ key >> 3) & 1) << 3 | (key & 3) << 1 | (key >> 3 & 1);
+}
 // Rotary parts are 128 bytes: two rows a pass's width.
 __device__ __forceinline__ int rope_swizzle(int key) { return key >> 1 & 7; }
 
@@ -850,13 +861,13 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         // the iteration before block 0 the weights and the output are zero.
         // a transposing read gives a lane its column (latent) of four rows (keys)
         const int tr_row = kBig ? 8 * (lane >> 5) + (c16 >> 2) : 4 * g + (c16 >> 2);
-        const int tr_col = (kBig ? 2 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
+        const int tr_col = (kBig ? 8 * (g & 1) : 0) + ((c16 & 3) >> 1);      // 16-byte chunk, + those of the tile
         const uint8_t* base[kLT][kBig ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < kLT; i++)
 #pragma unroll
           for (int h = 0; h < (kBig ? 2 : 1); h++)
-            base[i][h] = &sh.kv[buf].lat[tr_row + 4 * h][256 * y + 16 * ((kSize / 8 * i + tr_col) ^ swizzle(tr_row + 4 * h)) +
+            base[i][h] = &sh.kv[buf].lat[tr_row + 4 * h][256 * y + 16 * ((2 * i + tr_col) ^ swizzle(tr_row + 4 * h)) +
                                                          8 * (c16 & 1)];
         auto operand = [&](int u) {
           const int i = u % kLT, t = u / kLT;   // latent tile, keys
@@ -943,7 +954,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int q = 0; q < kAcc; q += 4) {
               const Acc v = acc[i][j];
-              const int lat = 128 * y + kSize * i + 2 * q + 4 * part;   // of v[q]
+              const int lat = latent_of(y, i, 2 * q + 4 * part);   // of v[q]
               *reinterpret_cast<uint2*>(os + (kSize * j + pr) * 2 * kLatent + ((2 * lat & ~15) ^ (16 * (pr & 15))) + (2 * lat & 15)) =
                   make_uint2(pack_bf16x2(v[q] * inv, v[q + 1] * inv), pack_bf16x2(v[q + 2] * inv, v[q + 3] * inv));
             }
@@ -1019,7 +1030,8 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
   const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane / kRowSize, c = lane & (kRowSize - 1);
   const int job = kTogether > 1 ? blockIdx.x : 4 * blockIdx.x + w;
   const int j = job / kQuads % kRT;   // row tile
-  const int lat = kRowSize * (job / (kQuads * kRT)) + 8 * (job % kQuads) + 4 * part;
+  constexpr int kLT = 128 / kRowSize;
+  const int tile_l = job / (kQuads * kRT), lat = latent_of(tile_l / kLT, tile_l % kLT, 8 * (job % kQuads) + 4 * part);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   for (int k0 = share.x + (kTogether > 1 ? w : 0); k0 <= share.y; k0 += kTogether * kDeep) {
