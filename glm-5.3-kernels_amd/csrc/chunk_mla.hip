@@ -51,22 +51,6 @@ constexpr int kTileCost = 10;       // what starting and ending a tile costs, in
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 16.f;      // how far (log2) a logit may pass its row's reference
 
-// n / d for any n, by multiplication.
-struct Divider {
-  uint32_t mul;
-  int sh1, sh2;
-};
-Divider divider(int64_t d) {
-  int log2_d = 0;   // rounded up
-  while ((INT64_C(1) << log2_d) < d) log2_d++;
-  const uint64_t mul = ((uint64_t(1) << log2_d) - static_cast<uint64_t>(d)) * (uint64_t(1) << 32) / static_cast<uint64_t>(d) + 1;
-  return {static_cast<uint32_t>(mul), log2_d < 1 ? log2_d : 1, log2_d > 1 ? log2_d - 1 : 0};
-}
-__device__ __forceinline__ int divide(uint32_t n, const Divider& d) {
-  const uint32_t t = __umulhi(d.mul, n);
-  return static_cast<int>((t + ((n - t) >> d.sh1)) >> d.sh2);
-}
-
 struct ChunkArgs {
   const uint16_t* q;
   int64_t sq_t, sq_h;

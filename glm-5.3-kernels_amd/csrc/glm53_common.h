@@ -55,6 +55,23 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   return mx(b[0], b[1]);
 }
 
+// n / d of 32-bit numbers by multiplication (Granlund and Montgomery's method):
+// with l = ceil(log2 d), mul = floor(2^32 (2^l - d) / d) + 1.
+struct Divider {
+  uint32_t mul;
+  int sh1, sh2;
+};
+inline Divider divider(int64_t d) {
+  int l = 0;
+  while ((INT64_C(1) << l) < d) l++;
+  const uint64_t mul = ((uint64_t(1) << l) - static_cast<uint64_t>(d)) * (uint64_t(1) << 32) / static_cast<uint64_t>(d) + 1;
+  return {static_cast<uint32_t>(mul), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divider& d) {
+  const uint32_t t = __umulhi(d.mul, n);
+  return (t + ((n - t) >> d.sh1)) >> d.sh2;
+}
+
 // Compute units of the current device (looked up once per device).
 inline int num_cus() {
   static std::atomic<int> cached[64];
