@@ -14,19 +14,22 @@
 // does not depend on the order in which they are taken.  Where all weights
 // are 0 the weights of p itself serve; where those are 0 too the token is -1.
 //
-// Two launches: every workgroup of the first decides its request (a few
-// dependent loads, the same for all of them) and sums the weights of its
-// chunk of the vocabulary; a workgroup of the second finds its request's
-// chunk and the token in it.  Bound by the latency of these chains for small
-// batches and by reading two rows of each request for large ones.
+// Two launches: every wave of the first decides its request (four dependent
+// loads, the same for all of them) and sums the weights of its 1024 entries of
+// the vocabulary, in whole numbers of 20 bits and 20 bits; a wave of the second
+// finds, from those sums, the 1024 entries that hold the token and the token in
+// them.  The target's own weights are summed only where the others are all 0,
+// by the eight waves of the second launch: they would double the first's
+// arithmetic, and draws from a distribution do not need them.
 #include "glm53_common.h"
 
 namespace glm53 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 16;
-constexpr int kChunk = kThreads * kPerThread;   // vocabulary entries of a workgroup
+constexpr int kPerLane = 16;
+constexpr int kChunk = 64 * kPerLane;      // vocabulary entries of a wave
+constexpr int kDrawWaves = 8;
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -44,22 +47,24 @@ struct VerifyArgs {
   int vocab, max_drafts, chunks;
   int32_t* tokens;       // [requests][max_drafts + 1]
   int32_t* accepted;
-  int64_t* sums;         // [requests][chunks][2]: of max(p - q, 0), of p
+  struct Decision* decisions;   // [requests]
+  uint64_t* sums;               // [requests][chunks]
 };
 
 __device__ __forceinline__ int64_t token_at(const VerifyArgs& a, int64_t i) {
   return a.ids_i64 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<int64_t>(static_cast<const int32_t*>(a.ids)[i]);
 }
 
-// floor(min(max(x, 0), 1) * 2^40), NaN as 0: the two products by 2^20 and the
-// remainder between them are exact.
-__device__ __forceinline__ uint64_t weight(float x) {
-  x = x > 0.f ? fminf(x, 1.f) : 0.f;
-  const float t = x * 1048576.f;
-  const uint32_t hi = static_cast<uint32_t>(t);
-  const uint32_t lo = static_cast<uint32_t>((t - static_cast<float>(hi)) * 1048576.f);
-  return (static_cast<uint64_t>(hi) << 20) + lo;
+// floor(min(max(x, 0), 1) * 2^40), NaN as 0, as hi * 2^20 + lo: the products by
+// 2^20 and the remainder between them are exact.
+struct Weight {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Weight weight(float x) {
+  const float t = fminf(fmaxf(x, 0.f), 1.f) * 1048576.f;
+  return {static_cast<uint32_t>(t), static_cast<uint32_t>(__builtin_amdgcn_fractf(t) * 1048576.f)};
 }
+__device__ __forceinline__ uint64_t weight_of(Weight w) { return (static_cast<uint64_t>(w.hi) << 20) + w.lo; }
 
 // What a request's rows say: how many drafts are taken, and whose weights the
 // next token is drawn from.
@@ -103,140 +108,158 @@ __device__ __forceinline__ Decision decide(const VerifyArgs& a, int r, int lane)
   return d;
 }
 
-// The weights of kPerThread entries from `at` of the decided row: of what is
-// left of the target (rest) and of the target itself (whole).
-__device__ __forceinline__ void load_weights(const VerifyArgs& a, const Decision& d, int at, uint64_t (&rest)[kPerThread],
-                                             uint64_t (&whole)[kPerThread]) {
+// Four entries from `at` on of what the next token is drawn from: of what is
+// left of the target's row, or (`whole`) of the row itself.
+struct Four {
+  float v[4];
+};
+__device__ __forceinline__ Four load_four(const VerifyArgs& a, const Decision& d, int at, bool whole) {
   const float* p = a.target + d.row * a.st;
-  const bool minus = d.place >= 0 && a.draft;
+  const bool minus = !whole && d.place >= 0 && a.draft;
   const float* q = minus ? a.draft + d.place * a.sd : nullptr;
-  float ps[kPerThread], qs[kPerThread];
-  if (at + kPerThread <= a.vocab) {
+  Four r;
+  if (at + 4 <= a.vocab) {
+    const f32x4u v = *reinterpret_cast<const f32x4u*>(p + at);
+    f32x4u u = {0.f, 0.f, 0.f, 0.f};
+    if (minus) u = *reinterpret_cast<const f32x4u*>(q + at);
 #pragma unroll
-    for (int k = 0; k < kPerThread; k += 4) {
-      const f32x4u v = *reinterpret_cast<const f32x4u*>(p + at + k);
-      ps[k] = v.x, ps[k + 1] = v.y, ps[k + 2] = v.z, ps[k + 3] = v.w;
-    }
-    if (minus) {
-#pragma unroll
-      for (int k = 0; k < kPerThread; k += 4) {
-        const f32x4u v = *reinterpret_cast<const f32x4u*>(q + at + k);
-        qs[k] = v.x, qs[k + 1] = v.y, qs[k + 2] = v.z, qs[k + 3] = v.w;
-      }
-    }
+    for (int k = 0; k < 4; k++) r.v[k] = v[k] - u[k];
   } else {
 #pragma unroll
-    for (int k = 0; k < kPerThread; k++) {
-      ps[k] = at + k < a.vocab ? p[at + k] : 0.f;
-      qs[k] = minus && at + k < a.vocab ? q[at + k] : 0.f;
-    }
+    for (int k = 0; k < 4; k++) r.v[k] = at + k < a.vocab ? minus ? p[at + k] - q[at + k] : p[at + k] : 0.f;
   }
+  if (!whole && d.place >= 0 && !a.draft) {
 #pragma unroll
-  for (int k = 0; k < kPerThread; k++) {
-    whole[k] = weight(ps[k]);
-    rest[k] = minus ? weight(ps[k] - qs[k]) : d.place >= 0 && at + k == d.token ? 0 : whole[k];
+    for (int k = 0; k < 4; k++) r.v[k] = at + k == d.token ? 0.f : r.v[k];
   }
+  return r;
 }
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+template <int kCtrl>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xf, 0xf, true));
 }
-
-__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
-  __shared__ uint64_t part[kThreads / 64][2];
-  const int r = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const Decision d = decide(a, r, lane);
-  if (d.row < 0) return;   // uniform
-  uint64_t rest[kPerThread], whole[kPerThread], s0 = 0, s1 = 0;
-  load_weights(a, d, blockIdx.x * kChunk + threadIdx.x * kPerThread, rest, whole);
-#pragma unroll
-  for (int k = 0; k < kPerThread; k++) s0 += rest[k], s1 += whole[k];
-  s0 = wave_sum_u64(s0), s1 = wave_sum_u64(s1);
-  if (lane == 0) part[w][0] = s0, part[w][1] = s1;
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    uint64_t s = 0;
-    for (int i = 0; i < kThreads / 64; i++) s += part[i][threadIdx.x];
-    a.sums[(static_cast<int64_t>(r) * a.chunks + blockIdx.x) * 2 + threadIdx.x] = static_cast<int64_t>(s);
-  }
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+  v = add_dpp<0xb1>(v);    // lanes 1 apart, 2 apart (quad_perm),
+  v = add_dpp<0x4e>(v);
+  v = add_dpp<0x141>(v);   // the other four of eight, the other eight of a row (mirrors)
+  v = add_dpp<0x140>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] + a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return b[0] + b[1];
 }
-
-// Inclusive scan over the workgroup.
-__device__ __forceinline__ uint64_t scan_u64(uint64_t v, uint64_t* part, int lane, int w, uint64_t& total) {
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {   // inclusive
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint64_t t = __shfl_up(v, d);
     if (lane >= d) v += t;
   }
-  __syncthreads();   // an earlier scan's reads of `part`
-  if (lane == 63) part[w] = v;
-  __syncthreads();
-  total = 0;
-  uint64_t before = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; i++) {
-    if (i < w) before += part[i];
-    total += part[i];
-  }
-  return v + before;
+  return v;
 }
 
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ uint64_t part[kThreads / 64];
-  __shared__ int found_chunk, found;
-  __shared__ uint64_t below;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const Decision d = decide(a, r, lane);
-  int32_t* out = a.tokens + static_cast<int64_t>(r) * (a.max_drafts + 1);
-  if (threadIdx.x == 0) found = -1;
-  int token = -1;
-  if (d.row >= 0) {
-    const int64_t* sums = a.sums + static_cast<int64_t>(r) * a.chunks * 2;
-    uint64_t total = 0;
-    int which = 0;
-    for (; which < 2; which++) {   // the rest's weights, else the target's
-      total = 0;
-      for (int i = threadIdx.x; i < a.chunks; i += kThreads) total += static_cast<uint64_t>(sums[2 * i + which]);
-      uint64_t all;
-      scan_u64(total, part, lane, w, all);
-      total = all;
-      if (total) break;
+// The sum of a wave's 1024 weights from `at` on.  1024 * 2^20 fits 32 bits.
+__device__ __forceinline__ uint64_t chunk_sum(const VerifyArgs& a, const Decision& d, int at, bool whole, int lane) {
+  Four v[kPerLane / 4];
+#pragma unroll
+  for (int k = 0; k < kPerLane / 4; k++) v[k] = load_four(a, d, at + 256 * k + 4 * lane, whole);
+  uint32_t hi = 0, lo = 0;
+#pragma unroll
+  for (int k = 0; k < kPerLane / 4; k++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const Weight t = weight(v[k].v[e]);
+      hi += t.hi, lo += t.lo;
     }
-    if (total) {
-      const double f = floor(a.sample_u[r] * static_cast<double>(total));
+  return weight_of({wave_sum_u32(hi), wave_sum_u32(lo)});
+}
+
+__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
+  const int r = blockIdx.y, lane = threadIdx.x & 63;
+  const int chunk = blockIdx.x * (kThreads / 64) + uniform(threadIdx.x >> 6);
+  if (chunk >= a.chunks) return;
+  const Decision d = decide(a, r, lane);
+  if (chunk == 0 && lane == 0) a.decisions[r] = d;
+  if (d.row < 0) return;
+  const uint64_t s = chunk_sum(a, d, chunk * kChunk, false, lane);
+  if (lane == 0) a.sums[static_cast<int64_t>(r) * a.chunks + chunk] = s;
+}
+
+// Where the running sum of `chunks` sums passes mark: the chunk, and the sum below it.
+struct Place {
+  int chunk;
+  uint64_t below;
+};
+__device__ __forceinline__ Place find_chunk(const uint64_t* sums, int chunks, uint64_t mark, int lane) {
+  uint64_t base = 0;
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    const uint64_t v = c0 + lane < chunks ? sums[c0 + lane] : 0;
+    const uint64_t upto = base + wave_scan_u64(v, lane);
+    const uint64_t past = __ballot(upto > mark);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      return {c0 + l, __shfl(upto - v, l)};
+    }
+    base = __shfl(upto, 63);
+  }
+  return {-1, 0};
+}
+
+__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const VerifyArgs a) {
+  __shared__ uint64_t part[kDrawWaves];
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  uint64_t* sums = a.sums + static_cast<int64_t>(r) * a.chunks;
+  uint64_t total = 0;
+  const Decision d = a.decisions[r];
+  const double s = a.sample_u[r];
+  int token = -1;
+  if (d.row >= 0) {   // uniform over the workgroup
+    for (int i = lane; i < a.chunks; i += 64) total += sums[i];
+    total = __shfl(wave_scan_u64(total, lane), 63);
+    const bool whole = total == 0 && d.place >= 0;
+    if (whole) {
+      // nothing is left: the target's own weights, into the sums of the others
+      __syncthreads();   // (which every wave has read)
+      for (int c = w; c < a.chunks; c += kDrawWaves) {
+        const uint64_t v = chunk_sum(a, d, c * kChunk, true, lane);
+        total += v;
+        if (lane == 0) sums[c] = v;
+      }
+      if (lane == 0) part[w] = total;
+      __syncthreads();   // and so are the sums in memory, for this workgroup
+      total = 0;
+      for (int i = 0; i < kDrawWaves; i++) total += part[i];
+    }
+    if (w == 0 && total) {
+      const double f = floor(s * static_cast<double>(total));
       uint64_t mark = f > 0. ? (f < static_cast<double>(total) ? static_cast<uint64_t>(f) : total - 1) : 0;
       if (mark >= total) mark = total - 1;
-      uint64_t base = 0;
-      for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
-        const int i = c0 + static_cast<int>(threadIdx.x);
-        const uint64_t v = i < a.chunks ? static_cast<uint64_t>(sums[2 * i + which]) : 0;
-        uint64_t all;
-        const uint64_t upto = base + scan_u64(v, part, lane, w, all);
-        if (upto > mark && upto - v <= mark) found_chunk = i, below = upto - v;
-        base += all;
-      }
-      __syncthreads();
-      const int at = found_chunk * kChunk + threadIdx.x * kPerThread;
-      uint64_t rest[kPerThread], whole[kPerThread], s = 0, all;
-      load_weights(a, d, at, rest, whole);
+      const Place at = find_chunk(sums, a.chunks, mark, lane);
+      // in the chunk (none only if the sums passed 64 bits): 16 entries a lane, in order
+      const int first = at.chunk < 0 ? a.vocab : at.chunk * kChunk + kPerLane * lane;
+      uint64_t v[kPerLane], sum = 0;
 #pragma unroll
-      for (int k = 0; k < kPerThread; k++) s += which ? whole[k] : rest[k];
-      uint64_t upto = below + scan_u64(s, part, lane, w, all) - s;
+      for (int k = 0; k < kPerLane; k += 4) {
+        const Four t = load_four(a, d, first + k, whole);
 #pragma unroll
-      for (int k = 0; k < kPerThread; k++) {
-        const uint64_t v = which ? whole[k] : rest[k];
-        if (upto <= mark && mark < upto + v) found = at + k;
-        upto += v;
+        for (int e = 0; e < 4; e++) sum += v[k + e] = weight_of(weight(t.v[e]));
       }
+      uint64_t upto = at.below + wave_scan_u64(sum, lane) - sum;
+      int found = -1;
+#pragma unroll
+      for (int k = 0; k < kPerLane; k++) {
+        if (upto <= mark && mark < upto + v[k]) found = first + k;
+        upto += v[k];
+      }
+      const uint64_t has = __ballot(found >= 0);
+      token = has ? __shfl(found, __builtin_ctzll(has)) : -1;
     }
   }
-  __syncthreads();
-  token = found;
-  for (int j = threadIdx.x; j <= a.max_drafts; j += kThreads)
+  if (w) return;
+  int32_t* out = a.tokens + static_cast<int64_t>(r) * (static_cast<int64_t>(a.max_drafts) + 1);
+  for (int64_t j = lane; j <= a.max_drafts; j += 64)
     out[j] = d.row < 0 || j > d.count ? -1 : j == d.count ? token : static_cast<int32_t>(token_at(a, d.first + j));
-  if (threadIdx.x == 0) a.accepted[r] = d.count;
+  if (lane == 0) a.accepted[r] = d.count;
 }
 
 }  // namespace
@@ -246,7 +269,7 @@ using namespace glm53;
 
 extern "C" int64_t glm53_verify_drafts_workspace_bytes(int64_t num_requests, int64_t vocab) {
   if (num_requests <= 0 || vocab <= 0) return 0;
-  return num_requests * ((vocab + kChunk - 1) / kChunk) * 16;
+  return num_requests * (static_cast<int64_t>(sizeof(Decision)) + (vocab + kChunk - 1) / kChunk * 8);
 }
 
 extern "C" int glm53_verify_drafts(const float* target_probs, int64_t st, int64_t num_rows, const float* draft_probs,
@@ -269,10 +292,12 @@ extern "C" int glm53_verify_drafts(const float* target_probs, int64_t st, int64_
   a.rows = num_rows, a.drafts = num_drafts;
   a.vocab = static_cast<int>(vocab), a.max_drafts = static_cast<int>(max_drafts);
   a.chunks = static_cast<int>((vocab + kChunk - 1) / kChunk);
-  a.tokens = tokens, a.accepted = accepted, a.sums = static_cast<int64_t*>(workspace);
+  a.tokens = tokens, a.accepted = accepted, a.decisions = static_cast<Decision*>(workspace);
+  a.sums = reinterpret_cast<uint64_t*>(a.decisions + num_requests);
   hipStream_t s = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
-  hipLaunchKernelGGL(verify_sums_kernel, dim3(a.chunks, static_cast<unsigned>(num_requests)), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(static_cast<unsigned>(num_requests)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(verify_sums_kernel, dim3((a.chunks + kThreads / 64 - 1) / (kThreads / 64), static_cast<unsigned>(num_requests)),
+                     dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(verify_draw_kernel, dim3(static_cast<unsigned>(num_requests)), dim3(64 * kDrawWaves), 0, s, a);
   return static_cast<int>(hipGetLastError());
 }
