@@ -68,7 +68,7 @@ inline Divider divider(int64_t d) {
   return {static_cast<uint32_t>(mul), l < 1 ? l : 1, l > 1 ? l - 1 : 0};
 }
 __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider& d) {
-  const uint32_t t = __umulhi(d.mul, n);
+  const uint32_t t = static_cast<uint32_t>(static_cast<uint64_t>(d.mul) * n >> 32);
   return (t + ((n - t) >> d.sh1)) >> d.sh2;
 }
 
