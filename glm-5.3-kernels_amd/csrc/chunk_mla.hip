@@ -265,6 +265,17 @@ __device__ __forceinline__ LateArgs* late_args() {
   return (LateArgs*)p;
 }
 
+// Brings the arguments into the scalar cache (a line of 64 bytes each), while
+// something else is waited for.
+__device__ __forceinline__ void touch_args() {
+  static_assert(sizeof(ChunkArgs) > 192 && sizeof(ChunkArgs) <= 256, "four lines");
+  uint32_t x, y, z;
+  asm volatile(
+      "s_load_dword %0, %3, 0x40\n\ts_load_dword %1, %3, 0x80\n\ts_load_dword %2, %3, 0xc0\n\ts_waitcnt lgkmcnt(0)"
+      : "=&s"(x), "=&s"(y), "=&s"(z)
+      : "s"(__builtin_amdgcn_kernarg_segment_ptr()));
+}
+
 // kRuns: pages of a multiple of eight rows, so that the eight rows of a block
 // that a wave brings in lie behind one another in one page.
 template <int kTM, bool kInt8, bool kSplit, bool kRuns>
@@ -300,9 +311,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     int units[kTiles], req[kTiles], sum = 0;
     Request of[kTiles];
     int* cu_s = reinterpret_cast<int*>(&sh.kv[0]);      // cu, then lens
-    for (int r = threadIdx.x; r <= a.num_reqs; r += kThreads) cu_s[r] = min(max(a.cu[r], 0), a.total_q);
     int* len_s = cu_s + kMaxSplitTiles + 16;
-    for (int r = threadIdx.x; r < a.num_reqs; r += kThreads) len_s[r] = a.lens[r];
+    // (both loads at once, and with them the arguments that come into use later)
+    static_assert(kMaxSplitTiles <= kThreads, "a request a thread");
+    const int rc = min(static_cast<int>(threadIdx.x), a.num_reqs), rl = min(static_cast<int>(threadIdx.x), a.num_reqs - 1);
+    const int cu_r = a.cu[rc], len_r = a.lens[rl], cu_end = a.cu[a.num_reqs];
+    touch_args();
+    cu_s[rc] = min(max(cu_r, 0), a.total_q);
+    len_s[rl] = len_r;
+    if (threadIdx.x == 0) cu_s[a.num_reqs] = min(max(cu_end, 0), a.total_q);
     wg_barrier();
 #pragma unroll
     for (int k = 0; k < kTiles; k++) {
