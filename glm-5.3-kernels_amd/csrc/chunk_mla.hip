@@ -77,7 +77,8 @@ struct ChunkArgs {
   float* lse;      // [total_q][heads], or null
   float* part;     // [2 * workgroups] slots of kTM x 512, accumulator order
   float2* ml;      // [2 * workgroups][kTM]: reference maximum (log2) and sum
-  int2* shares;    // [num_tiles]: first and last workgroup of a shared tile, or -1
+  int4* shares;    // [num_tiles]: of a shared tile its first and last workgroup, its first row over all
+                   // tokens and its rows, or -1
 };
 
 constexpr int kWaves = 8;
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     total = uniform(total), tiles = uniform(tiles);
     if (total == 0) {
       if (blockIdx.x == 0)
-        for (int t = threadIdx.x; t < a.num_tiles; t += kThreads) a.shares[t] = make_int2(-1, -1);
+        for (int t = threadIdx.x; t < a.num_tiles; t += kThreads) a.shares[t].x = -1;
       return;   // uniform over the workgroup
     }
     // A run of u blocks takes u times a block's time, and its partial (written,
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       upto_t += units[k];
       sh.ends[t] = upto_t;
       sh.reqs[t] = req[k];
-      if (blockIdx.x == 0 && t < a.num_tiles && units[k] == 0) a.shares[t] = make_int2(-1, -1);
+      if (blockIdx.x == 0 && t < a.num_tiles && units[k] == 0) a.shares[t].x = -1;
     }
     wg_barrier();
     const auto first = sh.first;
@@ -979,7 +980,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           e->ml[static_cast<int64_t>(slot) * kTM + lane] = make_float2(sh.alpha[lane], sum_of(lane));
         if (b0 == 0 && y == 0 && lane == 0) {
           const int longer = more * (each + 1);   // units of the longer runs
-          e->shares[tile] = make_int2(blockIdx.x, last_unit < longer ? last_unit / (each + 1) : more + (last_unit - longer) / each);
+          e->shares[tile] = make_int4(blockIdx.x, last_unit < longer ? last_unit / (each + 1) : more + (last_unit - longer) / each,
+                                       rq.t0 * a.heads + row0, min(rows - row0, kTM));
         }
       }
     }
@@ -1008,7 +1010,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
               l == 0.f ? -INFINITY : (sh.alpha[j] + __builtin_amdgcn_logf(l)) * kLn2;
         }
       }
-      if (kSplit && threadIdx.x == 0) e->shares[tile] = make_int2(-1, -1);
+      if (kSplit && threadIdx.x == 0) e->shares[tile].x = -1;
     }
     if (!kSplit) return;
   }
@@ -1022,12 +1024,13 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 template <int kTM, int kTogether>
 __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(const ChunkArgs a) {
   constexpr int kRowSize = ChunkShape<kTM>::kBig ? 32 : 16, kRT = kTM / kRowSize, kQuads = kRowSize == 32 ? 4 : 1;
-  constexpr int kDeep = 8;
+  constexpr int kDeep = kTogether > 1 ? 8 : 16;
   __shared__ float acc_s[kTogether][64][4];
   __shared__ float2 ml_s[kTogether][kRowSize];
   const int tile = blockIdx.y;
-  const int2 share = a.shares[tile];
+  const int4 share = a.shares[tile];
   if (share.x < 0) return;
+  const int first = uniform(share.x), last = uniform(share.y);
   const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane / kRowSize, c = lane & (kRowSize - 1);
   const int job = kTogether > 1 ? blockIdx.x : 4 * blockIdx.x + w;
   const int j = job / kQuads % kRT;   // row tile
@@ -1035,22 +1038,22 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
   const int tile_l = job / (kQuads * kRT), lat = latent_of(tile_l / kLT, tile_l % kLT, 8 * (job % kQuads) + 4 * part);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  for (int k0 = share.x + (kTogether > 1 ? w : 0); k0 <= share.y; k0 += kTogether * kDeep) {
+  for (int k0 = first + (kTogether > 1 ? w : 0); k0 <= last; k0 += kTogether * kDeep) {
     float2 ml[kDeep];
     f32x4 v[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; d++) {
-      const int k = min(k0 + kTogether * d, share.y);
-      const int64_t slot = 2 * static_cast<int64_t>(k) + (k == share.x);
-      ml[d] = a.ml[slot * kTM + kRowSize * j + c];
-      v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + job * 256 + 4 * lane);
+      const int k = k0 + kTogether * d;
+      ml[d] = make_float2(-INFINITY, 0.f), v[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (k <= last) {   // uniform
+        const int64_t slot = 2 * static_cast<int64_t>(k) + (k == first);
+        ml[d] = a.ml[slot * kTM + kRowSize * j + c];
+        v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + job * 256 + 4 * lane);
+      }
     }
     float top = m;
 #pragma unroll
-    for (int d = 0; d < kDeep; d++) {
-      if (k0 + kTogether * d > share.y) ml[d] = make_float2(-INFINITY, 0.f), v[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-      top = fmaxf(top, ml[d].x);
-    }
+    for (int d = 0; d < kDeep; d++) top = fmaxf(top, ml[d].x);
     const float base = top == -INFINITY ? 0.f : top;
     const float old = __builtin_amdgcn_exp2f(m - base);
     m = top;
@@ -1087,22 +1090,14 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
       for (int e = 0; e < 4; e++) acc[e] += f * v[e];
     }
   }
-  // the request of the tile
-  int at = 0;
-  for (int step = a.first_step; step; step >>= 1) {
-    const int r = at + step;
-    if (r < a.num_reqs && first_tile<kTM>(min(max(a.cu[r], 0), a.total_q), a.heads, r) <= tile) at = r;
-  }
-  const Request rq = request_of(a.cu[at], a.cu[at + 1], 0, a.total_q);
-  const int row = (tile - first_tile<kTM>(rq.t0, a.heads, at)) * kTM + kRowSize * j + c;
-  if (row >= rq.n * a.heads) return;
-  const int tok = divide(row, a.by_heads), head = row - tok * a.heads;
+  if (kRowSize * j + c >= share.w) return;
+  const int row = share.z + kRowSize * j + c, tok = divide(row, a.by_heads), head = row - tok * a.heads;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* o = a.out + static_cast<int64_t>(rq.t0 + tok) * a.so_t + static_cast<int64_t>(head) * a.so_h;
+  uint16_t* o = a.out + static_cast<int64_t>(tok) * a.so_t + static_cast<int64_t>(head) * a.so_h;
   *reinterpret_cast<uint2*>(o + lat) =
       make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   if (a.lse && lat == 0)
-    a.lse[static_cast<int64_t>(rq.t0 + tok) * a.heads + head] =
+    a.lse[static_cast<int64_t>(tok) * a.heads + head] =
         l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
@@ -1126,7 +1121,7 @@ Workspace workspace_of(int tm, int64_t tiles) {
   w.part = 0;
   w.ml = slots * tm * kLatent * 4;
   const int64_t shares = w.ml + slots * tm * 8;
-  w.bytes = shares + tiles * 8;
+  w.bytes = shares + tiles * 16;
   return w;
 }
 
@@ -1141,7 +1136,7 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
-    a.shares = reinterpret_cast<int2*>(p + ws.bytes - 8 * static_cast<int64_t>(a.num_tiles));
+    a.shares = reinterpret_cast<int4*>(p + ws.bytes - 16 * static_cast<int64_t>(a.num_tiles));
     hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a);
     // a shared tile has at most about CUs / tiles partials: 16 waves on a job
     // where that is many, four or one where it is few
