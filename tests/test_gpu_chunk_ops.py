@@ -60,6 +60,21 @@ def test_many_requests_on_long_contexts(cuda, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("news,lens,heads", [
+    ([150, 90, 0, 80, 60], [200, 170, 5, 80, 300], 64),
+    ([150, 90, 0, 80, 60], [1500, 1400, 5, 1300, 1450], 64),
+    ([1] * 300, [1 + 37 * (i % 40) for i in range(300)], 16),
+    ([2] * 300, [2000 if i == 7 else i % 3 for i in range(300)], 16),
+])
+def test_more_tiles_than_compute_units(cuda, news, lens, heads, int8):
+    from titan_mla import mla_chunk_attention_paged
+    a = make(cuda, 25, news, lens, heads, int8, 64)
+    log_case("chunk_mla tiles", len(news), heads, int8)
+    out, lse = mla_chunk_attention_paged(*a, SCALE, return_lse=True)
+    check(out, lse, *a)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
 @pytest.mark.parametrize("scale", [-0.03, 0.0, 1e-30])
 def test_scales(cuda, scale, int8):
     from titan_mla import mla_chunk_attention_paged
