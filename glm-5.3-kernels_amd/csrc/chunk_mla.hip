@@ -445,15 +445,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     // The queries come through LDS, laid out like keys, in the ring's buffers
     // that the first blocks leave: wave w brings in every eighth row.
     constexpr int kQBuf = kInt8 ? 1 : 2;
-    constexpr int kMine = kTM / kWaves, kQueryLoads = kInt8 ? kMine : 2 * kMine;
+    constexpr int kQueries = kTM / kWaves, kQueryLoads = kInt8 ? kQueries : 2 * kQueries;
     auto bring_queries = [&]() {
-      const int row = min(row0 + kWaves * min(c, kMine - 1) + w, rows - 1);   // (rows past the last: the last, not stored)
+      const int row = min(row0 + kWaves * min(c, kQueries - 1) + w, rows - 1);   // (rows past the last: the last, not stored)
       const int tok = divide(row, a.by_heads), head = row - tok * a.heads;
       const uint64_t at = reinterpret_cast<uint64_t>(a.q + static_cast<int64_t>(rq.t0 + tok) * a.sq_t +
                                                      static_cast<int64_t>(head) * a.sq_h);
       const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
 #pragma unroll
-      for (int j = 0; j < kMine; j++) {
+      for (int j = 0; j < kQueries; j++) {
         const uint8_t* from = reinterpret_cast<const uint8_t*>(
             static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, j)) |
             static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, j))) << 32);
@@ -466,6 +466,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       }
     };
 
+    // INT8: a block's conversion: kMine of a latent wave's eight rows by itself, kOthers by the rows' waves
+    constexpr int kMine = 4, kOthers = kOwn - kMine;
     // INT8: row 8 z + j of raw block `in`, and as bf16 into the block there
     // (without a row: any codes, with the scale 0)
     auto codes_of = [&](int in, int z, int j) {
@@ -578,14 +580,21 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
         for (int rt = 0; rt < kRQ; rt++) sum[rt] += part_sum[rt];
         if (n == count) break;
-        // INT8: half of the next block's conversion, between the products
+        // INT8: a part of the next block's conversion, between the products
         const int next = buf + 1 < kBufs ? buf + 1 : 0;
-        uint2 codes[kOwn / 2];
+        uint2 codes[kOthers];
+        if (kTM > 16) {
 #pragma unroll
-        for (int j = 0; j < kOwn / 2; j++) codes[j] = codes_of(next, w, kOwn / 2 + j);
-        if (!takes_rows) {
+          for (int j = 0; j < kOthers; j++) codes[j] = codes_of(next, w, kMine + j);
+        }
+        if (!takes_rows) {   // (of a 16-row tile: waves 2 and 3, each for two)
 #pragma unroll
-          for (int j = 0; j < kOwn / 2; j++) convert(next, w, kOwn / 2 + j, codes[j]);
+          for (int z = 0; z < 2; z++) {
+#pragma unroll
+            for (int j = 0; j < kOthers; j++) codes[j] = codes_of(next, 2 * kh + z, kMine + j);
+#pragma unroll
+            for (int j = 0; j < kOthers; j++) convert(next, 2 * kh + z, kMine + j, codes[j]);
+          }
         } else {
           const uint32_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v)));
           if constexpr (kInt8) {
@@ -605,7 +614,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++)
               t[rt][st % kSums] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], t[rt][st % kSums], 0, 0, 0);
-            if (st % 4 == 1 && st / 4 < kOwn / 2) convert(next, w, kOwn / 2 + st / 4, codes[st / 4]);
+            if (kTM > 16 && st % 4 == 1 && st / 4 < kOthers) convert(next, w, kMine + st / 4, codes[st / 4]);
             __builtin_amdgcn_sched_barrier(0);
           }
           float scale[4];
@@ -823,7 +832,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
           for (int q = 0; q < kAcc; q++) acc[i][j][q] = 0.f;
       wg_barrier();   // the queries have been read
 
-      // iteration n: PV of block n (the rows' waves are at block n + 1)
+      // iteration n: PV of block n (the rows' waves are at block n + 1).  Of
+      // 16-row tiles this side is the longer one, and goes first where both
+      // could (64 ragged INT8 requests 85.4 -> 81.8 us; 64-row tiles lose 6 %).
+      if (kTM == 16) __builtin_amdgcn_s_setprio(1);
       int buf = kBufs - 1;   // of block n
       for (int n = -1; n < count && count; n++) {
         const int next = buf + 1 < kBufs ? buf + 1 : 0, after = next + 1 < kBufs ? next + 1 : 0;
@@ -883,9 +895,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 #pragma unroll
           for (int u = 0; u < kRead; u++) v[u] = operand(u);
         }
-        uint2 codes[kOwn / 2];
+        uint2 codes[kMine];
 #pragma unroll
-        for (int j = 0; j < kOwn / 2; j++) codes[j] = codes_of(after, y, j);
+        for (int j = 0; j < kMine; j++) codes[j] = codes_of(after, y, j);
         if (n >= 0 && uniform(again) == n) {
           wg_barrier();   // the maxima
           wg_barrier();   // P
@@ -902,8 +914,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         const bool group = kRuns && ((n + kAhead + 1) & 63) == 32;
         if (group) look_up(n + kAhead + 1 + 32);
         auto between = [&](int u) {   // kPvSteps = 8
-          if (u < kOwn / 2) convert(after, y, u, codes[u]);
-          if (u == kOwn / 2) scales(after, masks);
+          if (u < kMine) convert(after, y, u, codes[u]);
+          if (u == kMine) scales(after, masks);
           if (u < kPairs) bring(into, u);
           if (u == 5 && !kRuns) look_up(n + kAhead + 3);
           if (u == 6) masks |= address(n + kAhead + 1) << (kInt8 ? 24 : 16);
@@ -938,6 +950,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
         wg_barrier();    // P
         buf = next;
       }
+      if (kTM == 16) __builtin_amdgcn_s_setprio(0);
       loads_left<0>();   // what was asked for past the last block
       wg_barrier();      // the sums
 
