@@ -155,16 +155,16 @@ def stream_handle(device) -> int:
 _here = contextlib.nullcontext()
 
 
-def on_device(device):
-    """torch.cuda.device(device), or nothing to enter where it is the current
+def on_device(index):
+    """torch.cuda.device(index), or nothing to enter where it is the current
     device already (the context costs a small call 2 us)."""
     import torch
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _here if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
-def raw_stream(device) -> int:
-    """stream_handle without the Stream object around it, where torch offers
-    that (1 us of a small call)."""
+def raw_stream(index) -> int:
+    """stream_handle of a device index without the Stream object around it,
+    where torch offers that (1 us of a small call)."""
     import torch
     get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(device.index) if get is not None else stream_handle(device)
+    return get(index) if get is not None else stream_handle(torch.device("cuda", index))

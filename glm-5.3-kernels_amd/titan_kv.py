@@ -58,21 +58,13 @@ def store_int8(x, cache, slots):
 _ROPE = 64
 
 
-def _aligned16(t):
-    """Whether t's rows can be read 16 bytes at a time: contiguous, every
-    other stride and the base a multiple of 16 bytes."""
-    size = t.element_size()
-    *steps, last = t.stride()
-    if last != 1 or t.data_ptr() % 16:
-        return False
-    for s in steps:
-        if s * size % 16:
-            return False
-    return True
-
-
 def _rows16(t):
-    return t if _aligned16(t) else t.clone(memory_format=torch.contiguous_format)
+    """bf16 t where its rows can be read 16 bytes at a time, else a copy."""
+    steps = t.stride()
+    odd = t.data_ptr() % 16 or steps[-1] != 1
+    for step in steps[:-1]:
+        odd = odd or step % 8
+    return t.clone(memory_format=torch.contiguous_format) if odd else t
 
 
 def store_rope(x, k_pe, positions, cos_sin, cache, slots, *, q_pe=None, q_out=None, norm_weight=None, eps=1e-6,
@@ -108,39 +100,51 @@ def store_rope(x, k_pe, positions, cos_sin, cache, slots, *, q_pe=None, q_out=No
     A token whose position is outside the table leaves its cache row as it
     was, and its queries become zeros.  Returns q_out (None without q_pe).
     """
-    if x.dim() != 2 or x.shape[1] != _LATENT or k_pe.dim() != 2 or k_pe.shape[1] != _ROPE:
-        raise ValueError(f"x must be [N, {_LATENT}] and k_pe [N, {_ROPE}], got {tuple(x.shape)} and {tuple(k_pe.shape)}")
-    if x.dtype != torch.bfloat16 or k_pe.dtype != torch.bfloat16 or cache.dtype != torch.bfloat16:
+    # (sizes, strides and addresses are taken once: a small call's time is this function's)
+    bf16, xs, ks, cs, ts = torch.bfloat16, x.shape, k_pe.shape, cache.shape, cos_sin.shape
+    if len(xs) != 2 or xs[1] != _LATENT or len(ks) != 2 or ks[1] != _ROPE:
+        raise ValueError(f"x must be [N, {_LATENT}] and k_pe [N, {_ROPE}], got {tuple(xs)} and {tuple(ks)}")
+    if x.dtype is not bf16 or k_pe.dtype is not bf16 or cache.dtype is not bf16:
         raise ValueError("x, k_pe and cache must be bf16")
-    if cache.dim() != 3 or cache.shape[2] != _LATENT + _ROPE or not _aligned16(cache):
+    page_step, row_step, step = cache.stride() if len(cs) == 3 else (0, 0, 0)
+    cache_ptr = cache.data_ptr()
+    if step != 1 or cs[2] != _LATENT + _ROPE or page_step % 8 or row_step % 8 or cache_ptr % 16:
         raise ValueError(f"cache must be [num_blocks, block_size, {_LATENT + _ROPE}] with contiguous 16-byte aligned rows")
-    if cos_sin.dim() != 2 or cos_sin.shape[1] != _ROPE or cos_sin.dtype not in (torch.float32, torch.bfloat16):
+    table_type = cos_sin.dtype
+    if len(ts) != 2 or ts[1] != _ROPE or (table_type is not torch.float32 and table_type is not bf16):
         raise ValueError(f"cos_sin must be fp32 or bf16 [max_pos, {_ROPE}]")
-    for name, t in (("positions", positions), ("slots", slots)):
-        if t.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-    N, n = x.shape[0], slots.numel()
-    if k_pe.shape[0] != N or positions.numel() != N or n > N:
-        raise ValueError(f"{N} latents, {k_pe.shape[0]} keys, {positions.numel()} positions and {n} slots")
-    if norm_weight is not None and (norm_weight.dtype != torch.bfloat16 or tuple(norm_weight.shape) != (_LATENT,)):
+    pos_type, slot_type = positions.dtype, slots.dtype
+    pos64, slot64 = pos_type is torch.int64, slot_type is torch.int64
+    if not (pos64 or pos_type is torch.int32) or not (slot64 or slot_type is torch.int32):
+        raise ValueError(f"positions and slots must be int32 or int64, got {pos_type} and {slot_type}")
+    N, n = xs[0], slots.numel()
+    if ks[0] != N or positions.numel() != N or n > N:
+        raise ValueError(f"{N} latents, {ks[0]} keys, {positions.numel()} positions and {n} slots")
+    if norm_weight is not None and (norm_weight.dtype is not bf16 or tuple(norm_weight.shape) != (_LATENT,)):
         raise ValueError(f"norm_weight must be bf16 [{_LATENT}]")
     if q_pe is None and q_out is not None:
         raise ValueError("q_out without q_pe")
-    dev = x.device
-    if not x.is_cuda or k_pe.device != dev or positions.device != dev or cos_sin.device != dev \
-            or cache.device != dev or slots.device != dev or (q_pe is not None and q_pe.device != dev) \
-            or (q_out is not None and q_out.device != dev) or (norm_weight is not None and norm_weight.device != dev):
+    index = x.get_device()
+    if index < 0 or k_pe.get_device() != index or positions.get_device() != index or cos_sin.get_device() != index \
+            or cache.get_device() != index or slots.get_device() != index \
+            or (q_pe is not None and q_pe.get_device() != index) or (q_out is not None and q_out.get_device() != index) \
+            or (norm_weight is not None and norm_weight.get_device() != index):
         raise ValueError("store_rope requires CUDA (HIP) tensors on one device")
-    heads = 0
+    heads = sq_t = sq_h = so_t = so_h = 0
+    q_ptr = out_ptr = norm_ptr = None
     if q_pe is not None:
-        if q_pe.dim() != 3 or q_pe.shape[0] != N or q_pe.shape[2] != _ROPE or q_pe.dtype != torch.bfloat16:
-            raise ValueError(f"q_pe must be bf16 [{N}, H, {_ROPE}], got {q_pe.dtype} {tuple(q_pe.shape)}")
-        heads = q_pe.shape[1]
+        qs = q_pe.shape
+        if len(qs) != 3 or qs[0] != N or qs[2] != _ROPE or q_pe.dtype is not bf16:
+            raise ValueError(f"q_pe must be bf16 [{N}, H, {_ROPE}], got {q_pe.dtype} {tuple(qs)}")
         if q_out is None:
-            q_out = torch.empty((N, heads, _ROPE), dtype=torch.bfloat16, device=dev)
-        elif q_out.dtype != torch.bfloat16 or q_out.shape != q_pe.shape or not _aligned16(q_out):
-            raise ValueError(f"q_out must be bf16 {tuple(q_pe.shape)} with contiguous 16-byte aligned rows")
-        q_pe = _rows16(q_pe)
+            q_out = torch.empty((N, qs[1], _ROPE), dtype=bf16, device=x.device)
+        so_t, so_h, step = q_out.stride() if q_out.dim() == 3 else (0, 0, 0)
+        out_ptr = q_out.data_ptr()
+        if q_out.dtype is not bf16 or q_out.shape != qs or step != 1 or so_t % 8 or so_h % 8 or out_ptr % 16:
+            raise ValueError(f"q_out must be bf16 {tuple(qs)} with contiguous 16-byte aligned rows")
+        q_pe, heads = _rows16(q_pe), qs[1]
+        sq_t, sq_h, _ = q_pe.stride()
+        q_ptr = q_pe.data_ptr()
     if n == 0:
         return q_out
     x, k_pe = _rows16(x), _rows16(k_pe)
@@ -148,19 +152,15 @@ def store_rope(x, k_pe, positions, cos_sin, cache, slots, *, q_pe=None, q_out=No
         cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
     if norm_weight is not None:
         norm_weight = _rows16(norm_weight)
+        norm_ptr = norm_weight.data_ptr()
     positions, slots = positions.contiguous(), slots.contiguous()
-    pages, block, _ = cache.shape
-    sq_t, sq_h = q_pe.stride()[:2] if heads else (0, 0)
-    so_t, so_h = q_out.stride()[:2] if heads else (0, 0)
     L = _lib.load()
-    with _lib.on_device(dev):
+    with _lib.on_device(index):
         rc = L.glm53_store_rope(
-            x.data_ptr(), x.stride(0), k_pe.data_ptr(), k_pe.stride(0), positions.data_ptr(),
-            positions.dtype == torch.int64, cos_sin.data_ptr(), cos_sin.dtype == torch.float32, cos_sin.shape[0],
-            bool(interleaved), norm_weight.data_ptr() if norm_weight is not None else None, eps, cache.data_ptr(),
-            2 * cache.stride(0), 2 * cache.stride(1), max(block, 1), pages * block, slots.data_ptr(),
-            slots.dtype == torch.int64, n, q_pe.data_ptr() if heads else None, sq_t, sq_h,
-            q_out.data_ptr() if heads else None, so_t, so_h, heads, _lib.raw_stream(dev))
+            x.data_ptr(), x.stride(0), k_pe.data_ptr(), k_pe.stride(0), positions.data_ptr(), pos64, cos_sin.data_ptr(),
+            table_type is torch.float32, ts[0], bool(interleaved), norm_ptr, eps, cache_ptr, 2 * page_step, 2 * row_step,
+            max(cs[1], 1), cs[0] * cs[1], slots.data_ptr(), slot64, n, q_ptr, sq_t, sq_h, out_ptr, so_t, so_h, heads,
+            _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "glm53_store_rope")
     return q_out

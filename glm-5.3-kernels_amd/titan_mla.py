@@ -397,41 +397,41 @@ def mla_chunk_attention_paged(
     Returns out, or (out, lse).  A token that sees no position gets zeros and
     -inf; rows of tokens at and past cu_seqlens_q[R] are not written.
     """
-    if q.dim() != 3 or kv_cache.dim() != 3:
-        raise ValueError(f"q must be [T, H, D] and kv_cache [num_blocks, block_size, width], got {tuple(q.shape)}, "
-                         f"{tuple(kv_cache.shape)}")
-    int8 = kv_cache.dtype == torch.int8
-    width, dim = (_ROW_BYTES, _BLOCK_DMODEL) if int8 else (_DIM_QK, _DIM_QK)
-    if not int8 and kv_cache.dtype != torch.bfloat16:
+    # (sizes, strides and addresses are taken once: a small call's time is this function's)
+    bf16, int32, qs, ks, ts = torch.bfloat16, torch.int32, q.shape, kv_cache.shape, block_table.shape
+    if len(qs) != 3 or len(ks) != 3:
+        raise ValueError(f"q must be [T, H, D] and kv_cache [num_blocks, block_size, width], got {tuple(qs)}, {tuple(ks)}")
+    int8 = kv_cache.dtype is torch.int8
+    width, dim, size = (_ROW_BYTES, _BLOCK_DMODEL, 1) if int8 else (_DIM_QK, _DIM_QK, 2)
+    if not int8 and kv_cache.dtype is not bf16:
         raise ValueError(f"kv_cache must be bf16 or int8, got {kv_cache.dtype}")
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not bf16:
         raise ValueError(f"q must be bf16, got {q.dtype}")
-    T, H, D = q.shape
-    if D != dim or kv_cache.shape[2] != width:
-        raise ValueError(f"a {kv_cache.dtype} cache has rows of {width} and queries of {dim}, got {kv_cache.shape[2]} "
-                         f"and {D}")
-    if H < 1 or kv_cache.shape[1] < 1:
+    (T, H, D), (pages, block, W) = qs, ks
+    if D != dim or W != width:
+        raise ValueError(f"a {kv_cache.dtype} cache has rows of {width} and queries of {dim}, got {W} and {D}")
+    if H < 1 or block < 1:
         raise ValueError("at least one head and one row per page")
-    if cu_seqlens_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.dtype != torch.int32:
+    if cu_seqlens_q.dtype is not int32 or seq_lens.dtype is not int32 or block_table.dtype is not int32:
         raise ValueError("cu_seqlens_q, seq_lens and block_table must be int32")
     R = seq_lens.numel()
-    if seq_lens.dim() != 1 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != R + 1 or block_table.dim() != 2 \
-            or block_table.shape[0] != R:
+    if seq_lens.dim() != 1 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() != R + 1 or len(ts) != 2 or ts[0] != R:
         raise ValueError(f"cu_seqlens_q must be [{R + 1}] and block_table [{R}, max_blocks] for seq_lens [{R}]")
-    dev = q.device
-    if not q.is_cuda or kv_cache.device != dev or cu_seqlens_q.device != dev or seq_lens.device != dev \
-            or block_table.device != dev:
+    index = q.get_device()
+    if index < 0 or kv_cache.get_device() != index or cu_seqlens_q.get_device() != index \
+            or seq_lens.get_device() != index or block_table.get_device() != index:
         raise ValueError("mla_chunk_attention_paged requires CUDA (HIP) tensors on one device")
-    size = 1 if int8 else 2
     page_step, row_step, step = kv_cache.stride()
     page_bytes, row_bytes, kv_ptr = page_step * size, row_step * size, kv_cache.data_ptr()
     if step != 1 or page_bytes % 16 or row_bytes % 16 or row_bytes < width * size or kv_ptr % 16:
         raise ValueError("cache rows must be contiguous, 16-byte aligned, their strides multiples of 16 bytes")
+    dev = q.device
     if out is None:
-        out = torch.empty((T, H, _BLOCK_DV), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, H, _BLOCK_DV) or out.device != dev \
+        out = torch.empty((T, H, _BLOCK_DV), dtype=bf16, device=dev)
+    elif out.dtype is not bf16 or tuple(out.shape) != (T, H, _BLOCK_DV) or out.get_device() != index \
             or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 or out.data_ptr() % 8:
         raise ValueError(f"out must be bf16 [{T}, {H}, {_BLOCK_DV}] on q's device, rows contiguous and 8-byte aligned")
+    so_t, so_h, _ = out.stride()
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T == 0 or R == 0:
         return (out, lse) if return_lse else out
@@ -439,23 +439,21 @@ def mla_chunk_attention_paged(
     if step != 1 or sq_h % 8 or sq_t % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         sq_t, sq_h, _ = q.stride()
-    if block_table.stride(1) != 1:
+    bt_step, step = block_table.stride()
+    if step != 1:
         block_table = block_table.contiguous()
-    if cu_seqlens_q.stride(0) != 1:
-        cu_seqlens_q = cu_seqlens_q.contiguous()
-    if seq_lens.stride(0) != 1:
-        seq_lens = seq_lens.contiguous()
+        bt_step = block_table.stride(0)
+    cu_seqlens_q, seq_lens = cu_seqlens_q.contiguous(), seq_lens.contiguous()
 
     L = _lib.load()
-    with _lib.on_device(dev):
-        ws_bytes = _chunk_workspace_bytes(T, R, H, dev.index)
+    with _lib.on_device(index):
+        ws_bytes = _chunk_workspace_bytes(T, R, H, index)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = L.glm53_chunk_mla(
-            q.data_ptr(), sq_t, sq_h, kv_ptr, int8, page_bytes, row_bytes, kv_cache.shape[0], kv_cache.shape[1],
-            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), R, block_table.stride(0),
-            block_table.shape[1], T, H, sm_scale, workspace.data_ptr() if ws_bytes else None, ws_bytes,
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None,
-            _lib.raw_stream(dev))
+            q.data_ptr(), sq_t, sq_h, kv_ptr, int8, page_bytes, row_bytes, pages, block, cu_seqlens_q.data_ptr(),
+            seq_lens.data_ptr(), block_table.data_ptr(), R, bt_step, ts[1], T, H, sm_scale,
+            workspace.data_ptr() if ws_bytes else None, ws_bytes, out.data_ptr(), so_t, so_h,
+            lse.data_ptr() if return_lse else None, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "glm53_chunk_mla")
     return (out, lse) if return_lse else out

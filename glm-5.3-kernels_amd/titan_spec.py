@@ -52,49 +52,54 @@ def verify_drafts(target_probs: torch.Tensor, draft_ids: torch.Tensor, draft_pro
     batch), or whose rows lie outside target_probs or draft_ids, has only -1 and
     0; the drawn token is -1 where the target's row has no weight either.
     """
-    if target_probs.dim() != 2 or target_probs.dtype != torch.float32 or target_probs.shape[1] < 1:
-        raise ValueError(f"target_probs must be fp32 [rows, vocab], got {target_probs.dtype} {tuple(target_probs.shape)}")
-    rows, vocab = target_probs.shape
-    if draft_ids.dtype not in (torch.int32, torch.int64) or draft_ids.dim() != 1:
+    # (sizes, strides and addresses are taken once: a small call's time is this function's)
+    ps, id_type = target_probs.shape, draft_ids.dtype
+    if len(ps) != 2 or target_probs.dtype is not torch.float32 or ps[1] < 1:
+        raise ValueError(f"target_probs must be fp32 [rows, vocab], got {target_probs.dtype} {tuple(ps)}")
+    rows, vocab = ps
+    ids64 = id_type is torch.int64
+    if not (ids64 or id_type is torch.int32) or draft_ids.dim() != 1:
         raise ValueError("draft_ids must be int32 or int64 [D]")
-    D = draft_ids.numel()
-    if draft_probs is not None and (draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (D, vocab)):
+    D, R = draft_ids.numel(), cu_rows.numel() - 1
+    if draft_probs is not None and (draft_probs.dtype is not torch.float32 or tuple(draft_probs.shape) != (D, vocab)):
         raise ValueError(f"draft_probs must be fp32 [{D}, {vocab}]")
-    if cu_rows.dtype != torch.int32 or cu_rows.dim() != 1 or cu_rows.numel() < 1:
+    if cu_rows.dtype is not torch.int32 or cu_rows.dim() != 1 or R < 0:
         raise ValueError("cu_rows must be int32 [R + 1]")
-    R = cu_rows.numel() - 1
-    if accept_u.dtype != torch.float32 or tuple(accept_u.shape) != (D,):
+    if accept_u.dtype is not torch.float32 or accept_u.dim() != 1 or accept_u.numel() != D:
         raise ValueError(f"accept_u must be fp32 [{D}]")
-    if sample_u.dtype != torch.float64 or tuple(sample_u.shape) != (R,):
+    if sample_u.dtype is not torch.float64 or sample_u.dim() != 1 or sample_u.numel() != R:
         raise ValueError(f"sample_u must be fp64 [{R}]")
     if max_drafts < 0:
         raise ValueError(f"max_drafts must be >= 0, got {max_drafts}")
     if R > _MAX_REQUESTS_PER_CALL:
         raise ValueError(f"at most {_MAX_REQUESTS_PER_CALL} requests per call, got {R}")
-    dev = target_probs.device
-    if not target_probs.is_cuda or draft_ids.device != dev or cu_rows.device != dev or accept_u.device != dev \
-            or sample_u.device != dev or (draft_probs is not None and draft_probs.device != dev):
+    index = target_probs.get_device()
+    if index < 0 or draft_ids.get_device() != index or cu_rows.get_device() != index \
+            or accept_u.get_device() != index or sample_u.get_device() != index \
+            or (draft_probs is not None and draft_probs.get_device() != index):
         raise ValueError("verify_drafts requires CUDA (HIP) tensors on one device")
+    dev = target_probs.device
     tokens = torch.empty((R, max_drafts + 1), dtype=torch.int32, device=dev)
     accepted = torch.empty(R, dtype=torch.int32, device=dev)
     if R == 0:
         return tokens, accepted
     if target_probs.stride(1) != 1:
         target_probs = target_probs.contiguous()
-    with_probs = draft_probs is not None and D > 0
-    if with_probs and draft_probs.stride(1) != 1:
-        draft_probs = draft_probs.contiguous()
+    draft_ptr, draft_step = None, 0
+    if draft_probs is not None and D > 0:
+        if draft_probs.stride(1) != 1:
+            draft_probs = draft_probs.contiguous()
+        draft_ptr, draft_step = draft_probs.data_ptr(), draft_probs.stride(0)
     draft_ids, cu_rows = draft_ids.contiguous(), cu_rows.contiguous()
     accept_u, sample_u = accept_u.contiguous(), sample_u.contiguous()
     L = _lib.load()
-    with _lib.on_device(dev):
+    with _lib.on_device(index):
         ws_bytes = _workspace_bytes(R, vocab)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         rc = L.glm53_verify_drafts(
-            target_probs.data_ptr(), target_probs.stride(0), rows, draft_probs.data_ptr() if with_probs else None,
-            draft_probs.stride(0) if with_probs else 0, draft_ids.data_ptr(), draft_ids.dtype == torch.int64, D,
+            target_probs.data_ptr(), target_probs.stride(0), rows, draft_ptr, draft_step, draft_ids.data_ptr(), ids64, D,
             cu_rows.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), R, vocab, max_drafts, workspace.data_ptr(),
-            ws_bytes, tokens.data_ptr(), accepted.data_ptr(), _lib.raw_stream(dev))
+            ws_bytes, tokens.data_ptr(), accepted.data_ptr(), _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "glm53_verify_drafts")
     return tokens, accepted
