@@ -257,11 +257,15 @@ __device__ __forceinline__ int last_key(const Request& r, int row0, int heads, c
   return k < 0 ? -1 : static_cast<int>(k < max_pos ? k : max_pos - 1);
 }
 
+// The arguments of the kernel's first loads lead (they come preloaded in
+// registers), the others follow in a struct this many bytes later.
+constexpr int kLeading = 24;
+
 // The kernel's arguments read where they are used, instead of being kept in
 // scalar registers from the start.
 typedef const __attribute__((address_space(4))) ChunkArgs LateArgs;
 __device__ __forceinline__ LateArgs* late_args() {
-  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr() + kLeading;
   asm volatile("" : "+s"(p));
   return (LateArgs*)p;
 }
@@ -269,7 +273,7 @@ __device__ __forceinline__ LateArgs* late_args() {
 // Brings the arguments into the scalar cache (a line of 64 bytes each), while
 // something else is waited for.
 __device__ __forceinline__ void touch_args() {
-  static_assert(sizeof(ChunkArgs) > 192 && sizeof(ChunkArgs) <= 256, "four lines");
+  static_assert(sizeof(ChunkArgs) + kLeading > 192 && sizeof(ChunkArgs) + kLeading <= 256, "four lines");
   uint32_t x, y, z;
   asm volatile(
       "s_load_dword %0, %3, 0x40\n\ts_load_dword %1, %3, 0x80\n\ts_load_dword %2, %3, 0xc0\n\ts_waitcnt lgkmcnt(0)"
@@ -280,7 +284,8 @@ __device__ __forceinline__ void touch_args() {
 // kRuns: pages of a multiple of eight rows, so that the eight rows of a block
 // that a wave brings in lie behind one another in one page.
 template <int kTM, bool kInt8, bool kSplit, bool kRuns>
-__global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs a) {
+__global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* cu, const int32_t* lens, int num_reqs,
+                                                                 int total_q, const ChunkArgs a) {
   using Shared = ChunkShared<kTM, kInt8>;
   constexpr bool kBig = ChunkShape<kTM>::kBig;
   constexpr int kRQ = kTM == 64 ? 2 : 1;           // QK: row tiles (of 16) of a wave
@@ -315,12 +320,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     int* len_s = cu_s + kMaxSplitTiles + 16;
     // (both loads at once, and with them the arguments that come into use later)
     static_assert(kMaxSplitTiles <= kThreads, "a request a thread");
-    const int rc = min(static_cast<int>(threadIdx.x), a.num_reqs), rl = min(static_cast<int>(threadIdx.x), a.num_reqs - 1);
-    const int cu_r = a.cu[rc], len_r = a.lens[rl], cu_end = a.cu[a.num_reqs];
+    const int rc = min(static_cast<int>(threadIdx.x), num_reqs), rl = min(static_cast<int>(threadIdx.x), num_reqs - 1);
+    const int cu_r = cu[rc], len_r = lens[rl], cu_end = cu[num_reqs];
     touch_args();
-    cu_s[rc] = min(max(cu_r, 0), a.total_q);
+    cu_s[rc] = min(max(cu_r, 0), total_q);
     len_s[rl] = len_r;
-    if (threadIdx.x == 0) cu_s[a.num_reqs] = min(max(cu_end, 0), a.total_q);
+    if (threadIdx.x == 0) cu_s[num_reqs] = min(max(cu_end, 0), total_q);
     wg_barrier();
 #pragma unroll
     for (int k = 0; k < kTiles; k++) {
@@ -328,9 +333,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       int at = 0;                                       // the last request that starts at or before tile t
       for (int step = a.first_step; step; step >>= 1) {
         const int r = at + step;
-        if (r < a.num_reqs && first_tile<kTM>(cu_s[r], a.heads, r) <= t) at = r;
+        if (r < num_reqs && first_tile<kTM>(cu_s[r], a.heads, r) <= t) at = r;
       }
-      const Request rq = request_of(cu_s[at], cu_s[at + 1], len_s[at], a.total_q);
+      const Request rq = request_of(cu_s[at], cu_s[at + 1], len_s[at], total_q);
       const int row0 = (t - first_tile<kTM>(rq.t0, a.heads, at)) * kTM;
       req[k] = at;
       of[k] = rq;
@@ -413,8 +418,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
     } else {
       // the last request that starts at or before this tile: its starts are in ascending order
       int begun = 0;
-      for (int i = threadIdx.x; i < a.num_reqs; i += kThreads)
-        begun += first_tile<kTM>(min(max(a.cu[i], 0), a.total_q), a.heads, i) <= tile;
+      for (int i = threadIdx.x; i < num_reqs; i += kThreads)
+        begun += first_tile<kTM>(min(max(cu[i], 0), total_q), a.heads, i) <= tile;
 #pragma unroll
       for (int d = 32; d; d >>= 1) begun += __shfl_xor(begun, d);
       if (lane == 0) sh.sums[w] = begun;
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
       for (int i = 0; i < kWaves; i++) r += sh.sums[i];
       r = uniform(max(r, 0));
     }
-    if (!known) rq = request_of(uniform(a.cu[r]), uniform(a.cu[r + 1]), uniform(a.lens[r]), a.total_q);
+    if (!known) rq = request_of(uniform(cu[r]), uniform(cu[r + 1]), uniform(lens[r]), total_q);
     const int rows = rq.n * a.heads;
     const int row0 = (tile - first_tile<kTM>(rq.t0, a.heads, r)) * kTM;
     if (!kSplit && (row0 < 0 || row0 >= rows)) return;   // an index between two requests
@@ -1035,13 +1040,14 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const ChunkArgs 
 // tiles, whose partials are many), or each of a workgroup's four waves takes a
 // job of its own.  kDeep partials are asked for at once.
 template <int kTM, int kTogether>
-__global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(const ChunkArgs a) {
+__global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(
+    const int4* shares, const float2* part_ml, const float* partials, const ChunkArgs a) {
   constexpr int kRowSize = ChunkShape<kTM>::kBig ? 32 : 16, kRT = kTM / kRowSize, kQuads = kRowSize == 32 ? 4 : 1;
   constexpr int kDeep = kTogether > 1 ? 8 : 16;
   __shared__ float acc_s[kTogether][64][4];
   __shared__ float2 ml_s[kTogether][kRowSize];
   const int tile = blockIdx.y;
-  const int4 share = a.shares[tile];
+  const int4 share = shares[tile];
   if (share.x < 0) return;
   const int first = uniform(share.x), last = uniform(share.y);
   const int w = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, part = lane / kRowSize, c = lane & (kRowSize - 1);
@@ -1060,8 +1066,8 @@ __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_ml
       ml[d] = make_float2(-INFINITY, 0.f), v[d] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (k <= last) {   // uniform
         const int64_t slot = 2 * static_cast<int64_t>(k) + (k == first);
-        ml[d] = a.ml[slot * kTM + kRowSize * j + c];
-        v[d] = *reinterpret_cast<const f32x4*>(a.part + slot * (kTM * kLatent) + job * 256 + 4 * lane);
+        ml[d] = part_ml[slot * kTM + kRowSize * j + c];
+        v[d] = *reinterpret_cast<const f32x4*>(partials + slot * (kTM * kLatent) + job * 256 + 4 * lane);
       }
     }
     float top = m;
@@ -1143,23 +1149,28 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
   // (units of all tiles are counted in an int)
   const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.block_size;
   if (a.num_tiles > kMaxSplitTiles || (cap / kKeys + 1 + kTileCost) * a.num_tiles > 0x7fffffff) {
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false, kRuns>), dim3(a.num_tiles), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, false, kRuns>), dim3(a.num_tiles), dim3(kThreads), 0, st,
+                       a.cu, a.lens, a.num_reqs, a.total_q, a);
   } else {
     const Workspace ws = workspace_of(kTM, a.num_tiles);
     uint8_t* p = static_cast<uint8_t*>(workspace);
     a.part = reinterpret_cast<float*>(p);
     a.ml = reinterpret_cast<float2*>(p + ws.ml);
     a.shares = reinterpret_cast<int4*>(p + ws.bytes - 16 * static_cast<int64_t>(a.num_tiles));
-    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a.cu,
+                       a.lens, a.num_reqs, a.total_q, a);
     // a shared tile has at most about CUs / tiles partials: 16 waves on a job
     // where that is many, four or one where it is few
     const int partials = num_cus() / a.num_tiles;
     if (partials > 64)
-      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 16>), dim3(2 * kTM, a.num_tiles), dim3(1024), 0, st, a);
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 16>), dim3(2 * kTM, a.num_tiles), dim3(1024), 0, st,
+                         a.shares, a.ml, a.part, a);
     else if (partials > 24)
-      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 4>), dim3(2 * kTM, a.num_tiles), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 4>), dim3(2 * kTM, a.num_tiles), dim3(256), 0, st,
+                         a.shares, a.ml, a.part, a);
     else
-      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 1>), dim3(kTM / 2, a.num_tiles), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 1>), dim3(kTM / 2, a.num_tiles), dim3(256), 0, st,
+                         a.shares, a.ml, a.part, a);
   }
   return static_cast<int>(hipGetLastError());
 }

@@ -146,23 +146,26 @@ __device__ __forceinline__ void store_rotated(uint16_t* o, int j, int interleave
   }
 }
 
+// (The arguments of the first loads lead: they come preloaded in registers.)
 template <int kRows, bool kStream>
-__global__ __launch_bounds__(64 * kWavesPerBlock) void store_rope_kernel(const RopeArgs a) {
+__global__ __launch_bounds__(64 * kWavesPerBlock) void store_rope_kernel(const void* positions, const void* slots, int64_t n,
+                                                                       const uint16_t* x, int64_t sx, int wide,
+                                                                       const RopeArgs a) {
   static_assert(kRows <= 8, "eight lanes a token's rotary key");
   const int lane = threadIdx.x & 63, part = blockIdx.y;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + uniform(threadIdx.x >> 6)) * kRows;
-  if (first >= a.n) return;
-  const int count = a.n - first < kRows ? static_cast<int>(a.n - first) : kRows;
+  if (first >= n) return;
+  const int count = n - first < kRows ? static_cast<int>(n - first) : kRows;
   const int j = lane & 7;
   if (part == 0) {
     // lanes 8 k .. 8 k + 7 look after token k (the last ones after the last)
     const int mine = min(lane >> 3, count - 1);
-    const int64_t pos = index_at(a.pos, a.pos_i64, first + mine);
-    const int64_t slot = index_at(a.slots, a.slots_i64, first + mine);
+    const int64_t pos = index_at(positions, wide & 1, first + mine);
+    const int64_t slot = index_at(slots, wide & 2, first + mine);
     u32x4 v[kRows], weight = {};
 #pragma unroll
     for (int k = 0; k < kRows; k++)
-      v[k] = load<kStream>(reinterpret_cast<const u32x4*>(a.x + (first + min(k, count - 1)) * a.sx + 8 * lane));
+      v[k] = load<kStream>(reinterpret_cast<const u32x4*>(x + (first + min(k, count - 1)) * sx + 8 * lane));
     if (a.norm) weight = *reinterpret_cast<const u32x4*>(a.norm + 8 * lane);
     Pairs key = {};
     if (lane < 8 * count) key = load_pairs<kStream>(a.k_pe + (first + mine) * a.sk, j, a.interleaved);
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void store_rope_kernel(const R
 #pragma unroll
   for (int k = 0; k < kRows; k++) {
     const int64_t tok = first + min(k, count - 1);
-    pos[k] = index_at(a.pos, a.pos_i64, tok);
+    pos[k] = index_at(positions, wide & 1, tok);
     q[k] = load_pairs<kStream>(a.q_pe + tok * a.sq_t + head * a.sq_h, j, a.interleaved);
   }
 #pragma unroll
@@ -226,7 +229,7 @@ int launch(const RopeArgs& a, hipStream_t st) {
   const unsigned parts = 1 + (a.heads + kHeadsPerWave - 1) / kHeadsPerWave;
   (void)hipGetLastError();
   hipLaunchKernelGGL((store_rope_kernel<kRows, kStream>), dim3(static_cast<unsigned>(grid), parts), dim3(64 * kWavesPerBlock), 0,
-                     st, a);
+                     st, a.pos, a.slots, a.n, a.x, a.sx, (a.pos_i64 ? 1 : 0) | (a.slots_i64 ? 2 : 0), a);
   return static_cast<int>(hipGetLastError());
 }
 

@@ -77,8 +77,8 @@ struct Decision {
 };
 
 // All 64 lanes of a wave call it and get the same answer.
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, int r, int lane) {
-  const int64_t c0 = a.cu[r], c1 = a.cu[r + 1];
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const int32_t* cu, int r, int lane) {
+  const int64_t c0 = cu[r], c1 = cu[r + 1];
   Decision d = {-1, -1, -1, c0 - r, 0};
   int64_t n = c1 - c0 - 1;
   if (n > a.max_drafts) n = a.max_drafts;
@@ -174,11 +174,12 @@ __device__ __forceinline__ uint64_t chunk_sum(const VerifyArgs& a, const Decisio
   return weight_of({wave_sum_u32(hi), wave_sum_u32(lo)});
 }
 
-__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
+// (The kernels' first loads' arguments lead: they come preloaded in registers.)
+__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const int32_t* cu, int chunks, const VerifyArgs a) {
   const int r = blockIdx.y, lane = threadIdx.x & 63;
   const int chunk = blockIdx.x * (kThreads / 64) + uniform(threadIdx.x >> 6);
-  if (chunk >= a.chunks) return;
-  const Decision d = decide(a, r, lane);
+  if (chunk >= chunks) return;
+  const Decision d = decide(a, cu, r, lane);
   if (chunk == 0 && lane == 0) a.decisions[r] = d;
   if (d.row < 0) return;
   const uint64_t s = chunk_sum(a, d, chunk * kChunk, false, lane);
@@ -205,22 +206,23 @@ __device__ __forceinline__ Place find_chunk(const uint64_t* sums, int chunks, ui
   return {-1, 0};
 }
 
-__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const Decision* decisions, const double* sample_u, uint64_t* all_sums,
+                                                                      int chunks, const VerifyArgs a) {
   __shared__ uint64_t part[kDrawWaves];
   const int r = blockIdx.x, lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
-  uint64_t* sums = a.sums + static_cast<int64_t>(r) * a.chunks;
+  uint64_t* sums = all_sums + static_cast<int64_t>(r) * chunks;
   uint64_t total = 0;
-  const Decision d = a.decisions[r];
-  const double s = a.sample_u[r];
+  const Decision d = decisions[r];
+  const double s = sample_u[r];
   int token = -1;
   if (d.row >= 0) {   // uniform over the workgroup
-    for (int i = lane; i < a.chunks; i += 64) total += sums[i];
+    for (int i = lane; i < chunks; i += 64) total += sums[i];
     total = __shfl(wave_scan_u64(total, lane), 63);
     const bool whole = total == 0 && d.place >= 0;
     if (whole) {
       // nothing is left: the target's own weights, into the sums of the others
       __syncthreads();   // (which every wave has read)
-      for (int c = w; c < a.chunks; c += kDrawWaves) {
+      for (int c = w; c < chunks; c += kDrawWaves) {
         const uint64_t v = chunk_sum(a, d, c * kChunk, true, lane);
         total += v;
         if (lane == 0) sums[c] = v;
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const Veri
       const double f = floor(s * static_cast<double>(total));
       uint64_t mark = f > 0. ? (f < static_cast<double>(total) ? static_cast<uint64_t>(f) : total - 1) : 0;
       if (mark >= total) mark = total - 1;
-      const Place at = find_chunk(sums, a.chunks, mark, lane);
+      const Place at = find_chunk(sums, chunks, mark, lane);
       // in the chunk (none only if the sums passed 64 bits): 16 entries a lane, in order
       const int first = at.chunk < 0 ? a.vocab : at.chunk * kChunk + kPerLane * lane;
       uint64_t v[kPerLane], sum = 0;
@@ -297,7 +299,8 @@ extern "C" int glm53_verify_drafts(const float* target_probs, int64_t st, int64_
   hipStream_t s = static_cast<hipStream_t>(stream);
   (void)hipGetLastError();
   hipLaunchKernelGGL(verify_sums_kernel, dim3((a.chunks + kThreads / 64 - 1) / (kThreads / 64), static_cast<unsigned>(num_requests)),
-                     dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(static_cast<unsigned>(num_requests)), dim3(64 * kDrawWaves), 0, s, a);
+                     dim3(kThreads), 0, s, a.cu, a.chunks, a);
+  hipLaunchKernelGGL(verify_draw_kernel, dim3(static_cast<unsigned>(num_requests)), dim3(64 * kDrawWaves), 0, s,
+                     a.decisions, a.sample_u, a.sums, a.chunks, a);
   return static_cast<int>(hipGetLastError());
 }
