@@ -462,7 +462,8 @@ int glm53_stream_probe(int kind, const void* src, void* dst, int64_t bytes, void
  *   out      bf16 [total_q, num_heads, 512], strides so_t, so_h (multiples of
  *            4 elements, 8-byte aligned); lse fp32 [total_q, num_heads] or
  *            NULL.
- * total_q * num_heads + 64 * num_reqs must stay below 2^31.
+ * total_q * num_heads + 64 * num_reqs must stay below 2^31.  Any block_size;
+ * multiples of 8 (rows less than 256 MB apart) are read faster.
  */
 int64_t glm53_chunk_mla_workspace_bytes(int64_t total_q, int64_t num_reqs, int64_t num_heads);
 int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h,
@@ -492,7 +493,8 @@ int glm53_chunk_mla(const void* q, int64_t sq_t, int64_t sq_h,
  *
  * A slot outside [0, capacity) is skipped (its queries are rotated); a
  * position outside [0, max_pos) leaves the cache as it was and gives zero
- * queries.  Slots of one call are distinct.  q_out may be q_pe.
+ * queries.  Slots of one call are distinct.  q_out may be q_pe.  capacity and
+ * block_size are below 2^32.
  * x, k_pe, q_pe, q_out: strides in elements; every base and stride a multiple
  * of 16 bytes, cos_sin (fp32 or bf16 [max_pos][64]) and norm_weight (bf16
  * [512] or NULL) contiguous and 16-byte aligned.
