@@ -34,6 +34,21 @@
 // into equal runs, one per workgroup; a tile that several workgroups share
 // leaves fp32 partials that the merge kernel joins.  Many tiles: one
 // workgroup each, longest first.
+//
+// Measured (inputs that no cache holds):
+//   * long chunks are bound by the products and the clock that the card holds
+//     beside them: 2048 tokens of 16 heads on 16k, 895 - 960 us, 1140 - 1220
+//     TFLOP/s (a large library product of plain matrices: 1225 - 1344).  A
+//     block of 32 keys and 64 rows takes 1900 cycles for 1088 of products a
+//     SIMD and 590 of LDS;
+//   * INT8 prompts also by the conversion, 52 instructions a wave and block:
+//     1234 tokens of 20 heads in five requests, 142 us, 640 TFLOP/s;
+//   * bf16 decode by memory: one request on 128k 42 us, 33 of them this kernel
+//     (4.6 TB/s with its start, 6.5 in its loop), 24 requests of up to four
+//     tokens 48 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
+//     requests 76 us);
+//   * small calls by their start: about 8 us of dependent loads (lengths,
+//     table, rows), scan and first block, then 4 for the merge's launch.
 #include <math.h>
 
 #include <type_traits>
@@ -47,6 +62,8 @@ constexpr int kLatent = 512;
 constexpr int kRope = 64;
 constexpr int kKeys = 32;           // keys per block
 constexpr int kMaxSplitTiles = 512; // most tiles whose blocks are cut into equal runs
+// Five INT8 prompts took 185 us with 2 here, 166 with 4, 154 with 7 and 10; 24
+// requests of four tokens 50, 49, 46 and 45.
 constexpr int kTileCost = 10;       // what starting and ending a tile costs, in blocks
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 16.f;      // how far (log2) a logit may pass its row's reference
@@ -371,7 +388,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
     }
     // A run of u blocks takes u times a block's time, and its partial (written,
     // read, joined) kTM / 1024 of that: the sum of both is least with
-    // sqrt(total * 1024 / kTM) runs.  No fewer than tiles: those come without partials.
+    // sqrt(total * 1024 / kTM) runs (one INT8 request on 2k: 15.9, 15.5 and 14.9
+    // us with 256, 512 and 1024 there; with 2048 one on 19k takes 25.8 instead
+    // of 24.5).  No fewer than tiles: those come without partials.
     const int best = max(tiles, static_cast<int>(sqrtf(static_cast<float>(total) * (1024 / kTM))));
     const int groups = min(min(static_cast<int>(gridDim.x), total), best), g = blockIdx.x;
     if (g >= groups) return;

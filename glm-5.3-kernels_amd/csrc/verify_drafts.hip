@@ -21,6 +21,13 @@
 // them.  The target's own weights are summed only where the others are all 0,
 // by the eight waves of the second launch: they would double the first's
 // arithmetic, and draws from a distribution do not need them.
+//
+// Bound by the chain of dependent loads and the two launches for small batches
+// (three drafts over 32000 tokens: 7.4 us, 4.0 and 3.8 the kernels alone), by
+// reading two rows of each request for large ones (64 requests over 131072: 67
+// MB in 16.3 us, 4.1 TB/s; 12.6 the sums).  A wave a chunk needs no barrier, and
+// 20 + 20 bits in 32-bit sums half the instructions of 64-bit ones: 10.6 and
+// 19.8 us before both.
 #include "glm53_common.h"
 
 namespace glm53 {
