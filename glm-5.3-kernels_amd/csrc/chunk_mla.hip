@@ -43,7 +43,7 @@
 //     SIMD and 590 of LDS;
 //   * INT8 prompts also by the conversion, 52 instructions a wave and block:
 //     1234 tokens of 20 heads in five requests, 142 us, 640 TFLOP/s;
-//   * bf16 decode by memory: one request on 128k 42 us, 33 of them this kernel
+//   * bf16 decode by memory: one request on 128k 41 us, 33 of them this kernel
 //     (4.6 TB/s with its start, 6.5 in its loop), 24 requests of up to four
 //     tokens 48 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
 //     requests 76 us);
@@ -221,6 +221,21 @@ __device__ __forceinline__ float quad_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Inclusive sum over the wave: within rows of 16 lanes by shifts, then the last
+// lane of row 0 (2) into row 1 (3) and that of row 1 into rows 2 and 3.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int add_from(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  return add_from<0x143, 0xc>(v);
+}
+
 // Eight INT8 codes as eight bf16 (exact): 12 instructions, all at the full rate.
 __device__ __forceinline__ uint4 codes_to_bf16(uint2 v) {
   uint32_t o[4];
@@ -361,12 +376,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
         units[k] = kTileCost + max(1, last_key<kTM>(rq, row0, a.heads, a.by_heads, max_pos) / kKeys + 1);
       sum += units[k];
     }
-    int upto = sum;                                     // inclusive scan over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
-    }
+    int upto = wave_scan(sum);                          // inclusive
     int filled = 0;
 #pragma unroll
     for (int k = 0; k < kTiles; k++) filled += __popcll(__ballot(units[k] > 0));
@@ -1062,7 +1072,7 @@ template <int kTM, int kTogether>
 __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(
     const int4* shares, const float2* part_ml, const float* partials, const ChunkArgs a) {
   constexpr int kRowSize = ChunkShape<kTM>::kBig ? 32 : 16, kRT = kTM / kRowSize, kQuads = kRowSize == 32 ? 4 : 1;
-  constexpr int kDeep = kTogether > 1 ? 8 : 16;
+  constexpr int kDeep = kTogether == 4 ? 8 : 16;
   __shared__ float acc_s[kTogether][64][4];
   __shared__ float2 ml_s[kTogether][kRowSize];
   const int tile = blockIdx.y;

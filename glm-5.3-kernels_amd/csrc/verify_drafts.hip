@@ -23,11 +23,12 @@
 // arithmetic, and draws from a distribution do not need them.
 //
 // Bound by the chain of dependent loads and the two launches for small batches
-// (three drafts over 32000 tokens: 7.4 us, 4.0 and 3.8 the kernels alone), by
+// (three drafts over 32000 tokens: 7.0 us, 4.2 and 3.0 the kernels alone), by
 // reading two rows of each request for large ones (64 requests over 131072: 67
-// MB in 16.3 us, 4.1 TB/s; 12.6 the sums).  A wave a chunk needs no barrier, and
+// MB in 15.7 us, 4.3 TB/s; 12.1 the sums).  A wave a chunk needs no barrier, and
 // 20 + 20 bits in 32-bit sums half the instructions of 64-bit ones: 10.6 and
-// 19.8 us before both.
+// 19.8 us before both.  Scans by lane shifts instead of LDS permutes: 7.4 and
+// 16.3 before.
 #include "glm53_common.h"
 
 namespace glm53 {
@@ -156,13 +157,25 @@ __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return b[0] + b[1];
 }
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {   // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t t = __shfl_up(v, d);
-    if (lane >= d) v += t;
-  }
-  return v;
+// Inclusive sum over the wave: within rows of 16 lanes by shifts, then the last
+// lane of row 0 (2) into row 1 (3) and that of row 1 into rows 2 and 3.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint64_t add_from(uint64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kCtrl, kRows, 0xf, true);
+  return v + (static_cast<uint32_t>(lo) | static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32);
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  return add_from<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {   // of a lane that is the same in all
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)) |
+         static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32;
 }
 
 // The sum of a wave's 1024 weights from `at` on.  1024 * 2^20 fits 32 bits.
@@ -202,13 +215,13 @@ __device__ __forceinline__ Place find_chunk(const uint64_t* sums, int chunks, ui
   uint64_t base = 0;
   for (int c0 = 0; c0 < chunks; c0 += 64) {
     const uint64_t v = c0 + lane < chunks ? sums[c0 + lane] : 0;
-    const uint64_t upto = base + wave_scan_u64(v, lane);
+    const uint64_t upto = base + wave_scan_u64(v);
     const uint64_t past = __ballot(upto > mark);
     if (past) {
       const int l = __builtin_ctzll(past);
-      return {c0 + l, __shfl(upto - v, l)};
+      return {c0 + l, lane_u64(upto - v, l)};
     }
-    base = __shfl(upto, 63);
+    base = lane_u64(upto, 63);
   }
   return {-1, 0};
 }
@@ -224,7 +237,7 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const Deci
   int token = -1;
   if (d.row >= 0) {   // uniform over the workgroup
     for (int i = lane; i < chunks; i += 64) total += sums[i];
-    total = __shfl(wave_scan_u64(total, lane), 63);
+    total = lane_u64(wave_scan_u64(total), 63);
     const bool whole = total == 0 && d.place >= 0;
     if (whole) {
       // nothing is left: the target's own weights, into the sums of the others
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const Deci
 #pragma unroll
         for (int e = 0; e < 4; e++) sum += v[k + e] = weight_of(weight(t.v[e]));
       }
-      uint64_t upto = at.below + wave_scan_u64(sum, lane) - sum;
+      uint64_t upto = at.below + wave_scan_u64(sum) - sum;
       int found = -1;
 #pragma unroll
       for (int k = 0; k < kPerLane; k++) {
@@ -261,7 +274,7 @@ __global__ __launch_bounds__(64 * kDrawWaves) void verify_draw_kernel(const Deci
         upto += v[k];
       }
       const uint64_t has = __ballot(found >= 0);
-      token = has ? __shfl(found, __builtin_ctzll(has)) : -1;
+      token = has ? __builtin_amdgcn_readlane(found, __builtin_ctzll(has)) : -1;
     }
   }
   if (w) return;
