@@ -127,7 +127,7 @@ struct __attribute__((aligned(16))) ChunkShared {
   std::conditional_t<kInt8, Int8Block, Bf16Block> kv[kBufs];
   uint8_t raw[kInt8 ? 3 : 0][kKeys][kLatent];   // INT8 rows as they are in the cache
   float raw_scale[kInt8 ? 3 : 0][kKeys];
-  float scl[kInt8 ? 3 : 0][kKeys];              // the scales, 0 for a key without a row
+  float4 scl[kInt8 ? 3 : 0][kKeys];             // what a key's scale s = f d comes to: scale_log2 s, log2 d, 1 / d, f
   uint8_t p[2][kTM][2 * kKeys];        // P, chunk c of 16 bytes of row r at c ^ (r / 4 % 4)
   int32_t page[kHalf * 64];            // block table entries of the coming blocks
   float red[2][kTM];                   // per key half: maxima; at the end the sums
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
       for (int rt = 0; rt < kRQ; rt++) ref[rt] = -3.4028234663852886e38f, sum[rt] = 0.f;
       f32x4 s[kRQ] = {};            // the last block's logits (log2)
       float part_sum[kRQ] = {};     // its part of the sums
-      float ksv[4] = {1.f, 1.f, 1.f, 1.f};
+      float4 ks[4] = {};            // INT8: the keys' scales
       // The weights of block n, for PV.
       auto weigh = [&](int n) {
 #pragma unroll
@@ -552,10 +552,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
           float p[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(s[rt][i] - ref[rt]);
-          part_sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
-          if constexpr (kInt8) {   // V = codes * scale: the scale goes to P
+          if constexpr (kInt8) {
+            // V = codes * f d.  The logits have log2 d in them, so that P has d
+            // (and the weight that counts most in a block is a power of two,
+            // which bf16 holds); the sum has not.
+            part_sum[rt] = (p[0] * ks[0].z + p[1] * ks[1].z) + (p[2] * ks[2].z + p[3] * ks[3].z);
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[i] *= ksv[i];
+            for (int i = 0; i < 4; i++) p[i] *= ks[i].w;
+          } else {
+            part_sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
           }
           // P is rounded to bf16 (like the output, 2^-9 of each weight on
           // the average); the sum keeps the unrounded weights.  With the
@@ -632,8 +637,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
         } else {
           const uint32_t have = static_cast<uint32_t>(uniform(static_cast<int>(have_v)));
           if constexpr (kInt8) {
-            const float4 v = *reinterpret_cast<const float4*>(&sh.scl[buf][16 * kh + 4 * g]);
-            ksv[0] = v.x, ksv[1] = v.y, ksv[2] = v.z, ksv[3] = v.w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) ks[i] = sh.scl[buf][16 * kh + 4 * g + i];
           }
           // two sums with one row tile, so that a product does not wait for the one before it
           constexpr int kSums = kRQ == 1 ? 2 : 1;
@@ -651,14 +656,13 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
             if (kTM > 16 && st % 4 == 1 && st / 4 < kOthers) convert(next, w, kMine + st / 4, codes[st / 4]);
             __builtin_amdgcn_sched_barrier(0);
           }
-          float scale[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) scale[i] = kInt8 ? a.scale_log2 * ksv[i] : a.scale_log2;
 #pragma unroll
           for (int rt = 0; rt < kRQ; rt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              s[rt][i] = (kSums == 1 ? t[rt][0][i] : t[rt][0][i] + t[rt][kSums - 1][i]) * scale[i];
+            for (int i = 0; i < 4; i++) {
+              const float dot = kSums == 1 ? t[rt][0][i] : t[rt][0][i] + t[rt][kSums - 1][i];
+              s[rt][i] = kInt8 ? __builtin_fmaf(dot, ks[i].x, ks[i].y) : dot * a.scale_log2;
+            }
           if (have != ~0u || (b0 + n + 1) * kKeys - 1 > least) {
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++) {
@@ -671,12 +675,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
                 if (key > limit || !(have >> key & 1)) s[rt][i] = -INFINITY;
               }
             }
-          }
-          if constexpr (kInt8) {
-            // a scale that is not a number has made its logits so; where it is
-            // masked, the weight 0 has to stay 0
-#pragma unroll
-            for (int i = 0; i < 4; i++) ksv[i] = fabsf(ksv[i]) < INFINITY ? ksv[i] : 0.f;
           }
           bool far = false;
 #pragma unroll
@@ -818,10 +816,20 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
             }
         }
       };
+      // INT8: scales s = f d.  d is |s| and f its sign where |s| is in the middle
+      // of fp32's range (2^-64 .. 2^64: then log2 d moves no weight out of it),
+      // else 1 and s; without a row, or with no number for a scale, f is 0: a
+      // masked weight 0 has to stay 0.
       auto scales = [&](int in, uint32_t mask) {
         if constexpr (kInt8) {
-          if (lane < kOwn)
-            sh.scl[in][kOwn * y + lane] = mask >> lane & 1 ? sh.raw_scale[in][kOwn * y + lane] : 0.f;
+          if (lane < kOwn) {
+            const float v = mask >> lane & 1 ? sh.raw_scale[in][kOwn * y + lane] : 0.f, size = fabsf(v);
+            const bool middle = size >= 0x1p-64f && size <= 0x1p64f;
+            const float d = middle ? size : 1.f;
+            sh.scl[in][kOwn * y + lane] =
+                make_float4(a.scale_log2 * v, __builtin_amdgcn_logf(d), __builtin_amdgcn_rcpf(d),
+                            middle ? copysignf(1.f, v) : size < INFINITY ? v : 0.f);
+          }
         }
       };
 

@@ -87,6 +87,34 @@ def test_scales(cuda, scale, int8):
     assert bool(((lse.double().cpu() - want_lse).abs() <= 2.0 ** -10).all())
 
 
+@pytest.mark.parametrize("heads", [16, 64])
+def test_key_scales_of_any_size(cuda, heads):
+    """INT8 rows whose scales are 0, negative, below any normal weight's range,
+    or (behind the last position) no numbers."""
+    from titan_mla import mla_chunk_attention_paged
+    q, cache, cu, lens, table = make(cuda, 26, [2, 1], [130, 45], heads, True, 64)
+    scale = cache[..., O.LATENT:O.LATENT + 4].contiguous().view(torch.float32)
+    for i, v in enumerate((0.0, -0.03, 1e-25, 1e-12, -1e-40, -0.0)):
+        scale.view(-1)[i::7] = torch.where(scale.view(-1)[i::7].isnan(), math.nan, v)
+    cache[..., O.LATENT:O.LATENT + 4] = scale.view(torch.int8)
+    log_case("chunk_mla key scales", heads)
+    out, lse = mla_chunk_attention_paged(q, cache, cu, lens, table, SCALE, return_lse=True)
+    check(out, lse, q, cache, cu, lens, table)
+
+
+@pytest.mark.parametrize("heads", [4, 16, 64])
+def test_one_key_is_that_key(cuda, heads):
+    """One visible key: its INT8 row times its scale, rounded once."""
+    from titan_mla import mla_chunk_attention_paged
+    a = make(cuda, 27, [1, 1, 1], [1, 1, 1], heads, True, 16)
+    log_case("chunk_mla one key", heads)
+    out = mla_chunk_attention_paged(*a, SCALE)
+    want = O.attend(*a, SCALE)[0]
+    # a value in [2^e, 2^(e + 1)) has bf16 neighbours 2^(e - 7) apart, so that rounding it is off by at most
+    # 2^(e - 8), 2^-8 of it; the scale's logarithm, power and quotient in fp32 add less than 2^-18
+    assert bool(((out.double().cpu() - want).abs() <= (2.0 ** -8 + 2.0 ** -18) * want.abs()).all())
+
+
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
 def test_a_row_that_turns_to_a_late_key(cuda, int8):
     """One row of a tile meets a key far above all before it, in a block where
