@@ -21,7 +21,7 @@
 //     each with the output in registers, and the loads.  bf16 rows come into a
 //     ring of four blocks in LDS by direct global -> LDS loads, three blocks
 //     ahead; INT8 rows as they are, four ahead, converted to bf16 once, two
-//     blocks before their use as V, a half by each kind.  Nothing waits for memory but the count of
+//     blocks before their use as V, by waves of both kinds.  Nothing waits for memory but the count of
 //     outstanding loads, once a block: the block table's entries come ahead too.
 // The softmax goes against a row's reference, which stays until a logit passes
 // it by 2^16 (in the first block, and seldom after it): then the block is
@@ -41,8 +41,8 @@
 //     TFLOP/s (a large library product of plain matrices: 1225 - 1344).  A
 //     block of 32 keys and 64 rows takes 1900 cycles for 1088 of products a
 //     SIMD and 590 of LDS;
-//   * INT8 prompts also by the conversion, 52 instructions a wave and block:
-//     1234 tokens of 20 heads in five requests, 142 us, 640 TFLOP/s;
+//   * INT8 prompts also by the conversion, 12 instructions for 8 codes: 1234
+//     tokens of 20 heads in five requests, 143 us, 630 TFLOP/s;
 //   * bf16 decode by memory: one request on 128k 41 us, 33 of them this kernel
 //     (4.6 TB/s with its start, 6.5 in its loop), 24 requests of up to four
 //     tokens 48 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
@@ -500,8 +500,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
       }
     };
 
-    // INT8: a block's conversion: kMine of a latent wave's eight rows by itself, kOthers by the rows' waves
-    constexpr int kMine = 4, kOthers = kOwn - kMine;
+    // INT8: a block's conversion: kMine of a latent wave's eight rows by itself,
+    // kOthers by the rows' waves (five prompts 147 us with 4 and 4, 143 with 3
+    // and 5; 16-row tiles 74.6 with 4 and 4 in the two waves without rows, 75.6
+    // with 3 and 5)
+    constexpr int kMine = kTM == 16 ? 4 : 3, kOthers = kOwn - kMine;
     // INT8: row 8 z + j of raw block `in`, and as bf16 into the block there
     // (without a row: any codes, with the scale 0)
     auto codes_of = [&](int in, int z, int j) {
@@ -640,6 +643,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
 #pragma unroll
             for (int i = 0; i < 4; i++) ks[i] = sh.scl[buf][16 * kh + 4 * g + i];
           }
+          static_assert(!kInt8 || (kSteps - 2) / 3 + 1 >= kOthers, "a step for each of the rows to convert");
           // two sums with one row tile, so that a product does not wait for the one before it
           constexpr int kSums = kRQ == 1 ? 2 : 1;
           f32x4 t[kRQ][kSums];
@@ -653,7 +657,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
 #pragma unroll
             for (int rt = 0; rt < kRQ; rt++)
               t[rt][st % kSums] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[st], qf[rt][st], t[rt][st % kSums], 0, 0, 0);
-            if (kTM > 16 && st % 4 == 1 && st / 4 < kOthers) convert(next, w, kMine + st / 4, codes[st / 4]);
+            if (kTM > 16 && st % 3 == 1 && st / 3 < kOthers) convert(next, w, kMine + st / 3, codes[st / 3]);
             __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
@@ -957,7 +961,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_mla_kernel(const int32_t* c
         if (group) look_up(n + kAhead + 1 + 32);
         auto between = [&](int u) {   // kPvSteps = 8
           if (u < kMine) convert(after, y, u, codes[u]);
-          if (u == kMine) scales(after, masks);
+          if (u == 7) scales(after, masks);
           if (u < kPairs) bring(into, u);
           if (u == 5 && !kRuns) look_up(n + kAhead + 3);
           if (u == 6) masks |= address(n + kAhead + 1) << (kInt8 ? 24 : 16);
