@@ -65,6 +65,8 @@ def test_many_requests_on_long_contexts(cuda, int8):
     ([150, 90, 0, 80, 60], [1500, 1400, 5, 1300, 1450], 64),
     ([1] * 300, [1 + 37 * (i % 40) for i in range(300)], 16),
     ([2] * 300, [2000 if i == 7 else i % 3 for i in range(300)], 16),
+    ([1] * 480, [i % 90 for i in range(480)], 1),     # as many requests as the split form takes
+    ([0] * 255 + [1] + [0] * 256, [5] * 255 + [70] + [5] * 256, 1),
 ])
 def test_more_tiles_than_compute_units(cuda, news, lens, heads, int8):
     from titan_mla import mla_chunk_attention_paged
