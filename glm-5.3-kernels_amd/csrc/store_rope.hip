@@ -250,7 +250,7 @@ extern "C" int glm53_store_rope(const void* x, int64_t x_row_stride, const void*
   // rows of a cache are counted in 32 bits (so many rows of 1152 bytes are 4.9 TB)
   if (capacity > 0xffffffffll || block_size > 0xffffffffll) return GLM53_ERR_BAD_SHAPE;
   if (n_slots == 0) return 0;
-  if (!x || !k_pe || !positions || !cos_sin || !cache || !slots || (num_heads && (!q_pe || !q_out)))
+  if (!x || !k_pe || !positions || (max_pos && !cos_sin) || (capacity && !cache) || !slots || (num_heads && (!q_pe || !q_out)))
     return GLM53_ERR_NULL_POINTER;
   const auto off = [](const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % 16 || n % 16; };
   if (off(x, 2 * x_row_stride) || off(k_pe, 2 * k_row_stride) || off(cos_sin, 0) || off(norm_weight, 0) ||

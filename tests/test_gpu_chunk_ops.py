@@ -165,6 +165,24 @@ def test_appending_many_tokens(cuda, n, heads):
         assert not q.cpu()[~known].any()
 
 
+def test_caches_and_tables_without_rows(cuda):
+    """No page, no position: nothing is stored or seen, queries without an
+    angle are zero."""
+    from titan_kv import store_rope
+    from titan_mla import mla_chunk_attention_paged
+    d = rope.make(cuda, 3, 4, 2, 16, 1, torch.float32)
+    log_case("empty cache")
+    q = store_rope(d["x"], d["k_pe"], d["positions"], d["cos_sin"], d["cache"][:0], d["slots"], q_pe=d["q_pe"])
+    assert rope.close(q, rope.reference(d, False, False)[1], 2 * d["q_pe"].abs().max().item())
+    before = d["cache"].clone()
+    q = store_rope(d["x"], d["k_pe"], d["positions"], d["cos_sin"][:0], d["cache"], d["slots"], q_pe=d["q_pe"])
+    assert not q.any() and torch.equal(before, d["cache"])
+    for int8 in (False, True):
+        q, cache, cu, lens, table = make(cuda, 28, [2, 1], [90, 20], 16, int8, 64)
+        out, lse = mla_chunk_attention_paged(q, cache[:0], cu, lens, table, SCALE, return_lse=True)
+        assert not out.any() and bool(torch.isneginf(lse).all())
+
+
 @pytest.mark.parametrize("vocab", [1023, 1024, 1025, 2049, 65537, 70001])
 @pytest.mark.parametrize("probs", [True, False], ids=["probs", "lookup"])
 def test_vocabularies_at_the_ends_of_chunks(cuda, vocab, probs):
