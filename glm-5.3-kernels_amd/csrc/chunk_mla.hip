@@ -45,7 +45,7 @@
 //     tokens of 20 heads in five requests, 143 us, 630 TFLOP/s;
 //   * bf16 decode by memory: one request on 128k 41 us, 33 of them this kernel
 //     (4.6 TB/s with its start, 6.5 in its loop), 24 requests of up to four
-//     tokens 48 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
+//     tokens 46 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
 //     requests 76 us);
 //   * small calls by their start: about 8 us of dependent loads (lengths,
 //     table, rows), scan and first block, then 4 for the merge's launch.
@@ -1084,7 +1084,7 @@ template <int kTM, int kTogether>
 __global__ __launch_bounds__(kTogether > 1 ? 64 * kTogether : 256) void chunk_mla_merge_kernel(
     const int4* shares, const float2* part_ml, const float* partials, const ChunkArgs a) {
   constexpr int kRowSize = ChunkShape<kTM>::kBig ? 32 : 16, kRT = kTM / kRowSize, kQuads = kRowSize == 32 ? 4 : 1;
-  constexpr int kDeep = kTogether == 4 ? 8 : 16;
+  constexpr int kDeep = kTogether == 4 ? 4 : 16;
   __shared__ float acc_s[kTogether][64][4];
   __shared__ float2 ml_s[kTogether][kRowSize];
   const int tile = blockIdx.y;
@@ -1201,12 +1201,13 @@ int launch(ChunkArgs& a, void* workspace, hipStream_t st) {
     hipLaunchKernelGGL((chunk_mla_kernel<kTM, kInt8, true, kRuns>), dim3(num_cus()), dim3(kThreads), 0, st, a.cu,
                        a.lens, a.num_reqs, a.total_q, a);
     // a shared tile has at most about CUs / tiles partials: 16 waves on a job
-    // where that is many, four or one where it is few
+    // where that is many, four or one where it is few (24 requests of 64 rows,
+    // about ten each: 47.7 us with one, 45.4 with four; 23 of 32 rows 21.3, 22.0)
     const int partials = num_cus() / a.num_tiles;
     if (partials > 64)
       hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 16>), dim3(2 * kTM, a.num_tiles), dim3(1024), 0, st,
                          a.shares, a.ml, a.part, a);
-    else if (partials > 24)
+    else if (partials > (kTM == 64 ? 4 : 24))
       hipLaunchKernelGGL((chunk_mla_merge_kernel<kTM, 4>), dim3(2 * kTM, a.num_tiles), dim3(256), 0, st,
                          a.shares, a.ml, a.part, a);
     else
