@@ -37,16 +37,16 @@
 //
 // Measured (inputs that no cache holds):
 //   * long chunks are bound by the products and the clock that the card holds
-//     beside them: 2048 tokens of 16 heads on 16k, 895 - 960 us, 1140 - 1220
+//     beside them: 2048 tokens of 16 heads on 16k, 895 - 968 us, 1130 - 1220
 //     TFLOP/s (a large library product of plain matrices: 1225 - 1344).  A
 //     block of 32 keys and 64 rows takes 1900 cycles for 1088 of products a
 //     SIMD and 590 of LDS;
 //   * INT8 prompts also by the conversion, 12 instructions for 8 codes: 1234
-//     tokens of 20 heads in five requests, 143 us, 630 TFLOP/s;
+//     tokens of 20 heads in five requests, 145 us, 620 TFLOP/s;
 //   * bf16 decode by memory: one request on 128k 41 us, 33 of them this kernel
 //     (4.6 TB/s with its start, 6.5 in its loop), 24 requests of up to four
-//     tokens 46 us; INT8 decode by the conversion and LDS (4.1 TB/s, 64 ragged
-//     requests 76 us);
+//     tokens 46 us; INT8 decode by the conversion and LDS (3.9 TB/s, 64 ragged
+//     requests 77 us);
 //   * small calls by their start: about 8 us of dependent loads (lengths,
 //     table, rows), scan and first block, then 4 for the merge's launch.
 #include <math.h>
